@@ -1,0 +1,366 @@
+"""Measured cases of the 8-bit paged KV cache: writing it, reading it back, and attention over it.
+
+The cache holds the K and V row of every (token, KV head) as head_dim e4m3 codes and one
+power-of-two scale (an e8m0 byte: exponent + 127), in pages of 16 tokens:
+codes [pages, 16, kv_heads, head_dim], scales [pages, kv_heads, 16].  The scale is the smallest
+2^e with max|row| <= 448 * 2^e (e >= -127), so a stored value is code * 2^e and dividing by the
+scale is exact: the codes do not depend on the precision they are computed in.
+
+Four operators ("op" of a case):
+  write     the new tokens of every request quantised into its pages, then read back
+  readback  ranges of cached tokens as dense, packed K and V
+  decode    one query token per request against its cached tokens
+  chunk     several new query tokens per request, causal, bottom-right aligned
+"""
+import math
+import random
+
+import torch
+
+own = False
+
+PAGE = 16
+E4M3_MAX = 448.0
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+# ---- cases -------------------------------------------------------------------
+# batch: requests; len_lo..len_hi: cached tokens of a request (new ones included), spread
+# over their logarithm; new_lo..new_hi: new tokens of a request (write, chunk) or tokens read
+# back; hq / hkv / d: query heads, KV heads, head_dim; dtype: of q, new K / V and the results.
+def listed():
+    return [
+        # one decode step's tokens of 32 requests go into the cache
+        dict(name="write step, 32 requests", op="write", batch=32, len_lo=4096, len_hi=8192, new_lo=1, new_hi=1,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # prompts of a ragged batch go into the cache
+        dict(name="write prompts, 8 ragged", op="write", batch=8, len_lo=700, len_hi=8191, new_lo=700, new_hi=8191,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # a 32K-token request leaves the cache as dense K and V, to be scored and compacted
+        dict(name="readback 32768", op="readback", batch=1, len_lo=32768, len_hi=32768, new_lo=32768, new_hi=32768,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # windows of a ragged batch, a smaller model's heads, half precision
+        dict(name="readback windows, d 64", op="readback", batch=24, len_lo=100, len_hi=4000, new_lo=33, new_hi=700,
+             hq=16, hkv=2, d=64, dtype="fp16"),
+        # the serving step that fills a pool: 32 requests of 4K to 32K tokens
+        dict(name="decode 32 x 4K-32K", op="decode", batch=32, len_lo=4096, len_hi=32768, new_lo=1, new_hi=1,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # one long document; its row sums are kept for a merge
+        dict(name="decode 1 x 131072", op="decode", batch=1, len_lo=131072, len_hi=131072, new_lo=1, new_hi=1,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # a few short chats: launches and latency
+        dict(name="decode 4 x 1-300", op="decode", batch=4, len_lo=1, len_hi=300, new_lo=1, new_hi=1,
+             hq=16, hkv=2, d=64, dtype="fp16"),
+        # wide heads, one query head to a KV head
+        dict(name="decode 12 x 500-9000, d 256", op="decode", batch=12, len_lo=500, len_hi=9000, new_lo=1, new_hi=1,
+             hq=8, hkv=8, d=256, dtype="bf16"),
+        # drafted tokens of 16 requests run through the model at once
+        dict(name="chunk 16 x 4 drafted", op="chunk", batch=16, len_lo=2000, len_hi=16000, new_lo=4, new_hi=4,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # chunked prefill of 8 requests beside decoding
+        dict(name="chunk 8 x 512", op="chunk", batch=8, len_lo=900, len_hi=16000, new_lo=512, new_hi=512,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # the last chunk of a long prompt
+        dict(name="chunk 2048 of 32768", op="chunk", batch=1, len_lo=32768, len_hi=32768, new_lo=2048, new_hi=2048,
+             hq=32, hkv=8, d=128, dtype="bf16"),
+        # ragged short chunks, a smaller model's heads, half precision
+        dict(name="chunk 6 ragged, d 64", op="chunk", batch=6, len_lo=50, len_hi=3000, new_lo=1, new_hi=333,
+             hq=16, hkv=2, d=64, dtype="fp16"),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(("write", "readback", "decode", "decode", "chunk", "chunk"))
+    hkv, n_rep = rng.choice(((8, 4), (2, 8), (8, 1), (4, 4), (1, 8), (3, 2), (2, 16), (5, 5)))
+    d = rng.choice((64, 128, 128, 128, 256))
+    dtype = rng.choice(("bf16", "bf16", "fp16"))
+    if op == "write" and rng.random() < 0.25:
+        dtype = "fp32"
+    if op == "decode":
+        hi = _log_int(rng, 1, 100000)
+        batch = _log_int(rng, 1, max(1, min(128, 800000000 // (hi * 2 * hkv * (d + 1)))))
+        lo, new_lo, new_hi = max(1, hi // rng.choice((1, 2, 10, 100))), 1, 1
+    elif op == "chunk":
+        hi = _log_int(rng, 1, 32768)
+        new_hi = min(hi, _log_int(rng, 1, max(1, min(2048, int(2e11 / (hkv * n_rep * d * hi))))))
+        batch = _log_int(rng, 1, max(1, min(32, int(2e11 / (hkv * n_rep * d * new_hi * hi)))))
+        lo, new_lo = max(1, hi // rng.choice((1, 3, 20))), max(0, new_hi // rng.choice((1, 2, 7)) - 1)
+    else:
+        hi = _log_int(rng, 1, 32768)
+        new_hi = 1 if op == "write" and rng.random() < 0.3 else hi
+        batch = _log_int(rng, 1, max(1, min(64, 65536 // hi)))
+        lo, new_lo = max(1, hi // rng.choice((1, 3, 20))), max(0, new_hi // rng.choice((1, 4)) - 1)
+    return dict(op=op, batch=batch, len_lo=lo, len_hi=hi, new_lo=new_lo, new_hi=new_hi, hq=hkv * n_rep, hkv=hkv, d=d,
+                dtype=dtype)
+
+
+def _lengths(case):
+    """Cached and new tokens of each request: of the case alone, so that work() knows them."""
+    rng = random.Random(repr(sorted((k, v) for k, v in case.items() if k != "name")))
+    lens = [_log_int(rng, case["len_lo"], case["len_hi"]) for _ in range(case["batch"])]
+    new = [min(n, rng.randint(case["new_lo"], case["new_hi"])) for n in lens]
+    lens[0] = case["len_hi"]
+    new[0] = min(lens[0], case["new_hi"])
+    return lens, new
+
+
+def _pages(n):
+    return -(-n // PAGE)
+
+
+# ---- inputs ------------------------------------------------------------------
+def _rows(gen, n, hkv, d, device):
+    """K or V rows as a model makes them: unit normal, a loud channel or two, tokens of unequal norm."""
+    x = torch.randn(n, hkv, d, generator=gen, device=device)
+    x *= torch.exp2(torch.randn(n, hkv, 1, generator=gen, device=device) * 0.5)
+    x[:, :, gen.initial_seed() % d] *= 3.0
+    return x
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    lens, new = _lengths(case)
+    B, hq, hkv, d, dtype = case["batch"], case["hq"], case["hkv"], case["d"], DTYPES[case["dtype"]]
+    need = [_pages(n) for n in lens]
+    n_pages = sum(need) + 3
+    # a cache that already holds every request's tokens, in pages in no order
+    k_codes = torch.empty(n_pages, PAGE, hkv, d, dtype=torch.float8_e4m3fn, device=dev)
+    v_codes = torch.empty_like(k_codes)
+    k_scales = torch.empty(n_pages, hkv, PAGE, dtype=torch.uint8, device=dev)
+    v_scales = torch.empty_like(k_scales)
+    at = 0
+    while at < n_pages:
+        n = min(4096, n_pages - at)
+        for codes, scales in ((k_codes, k_scales), (v_codes, v_scales)):
+            c, e = _quantise(_rows(gen, n * PAGE, hkv, d, dev))
+            codes[at:at + n] = c.view(n, PAGE, hkv, d)
+            scales[at:at + n] = e.view(n, PAGE, hkv).transpose(1, 2)
+        at += n
+    ids = torch.randperm(n_pages, generator=gen, device=dev).to(torch.int32)
+    table = torch.zeros(B, max(need), dtype=torch.int32, device=dev)
+    used = 0
+    for b, n in enumerate(need):
+        table[b, :n] = ids[used:used + n]
+        used += n
+    total, cu = sum(new), [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    state = dict(case=dict(case), k_codes=k_codes, v_codes=v_codes, k_scales=k_scales, v_scales=v_scales, table=table,
+                 lens=torch.tensor(lens, dtype=torch.int32, device=dev),
+                 cu=torch.tensor(cu, dtype=torch.int32, device=dev),
+                 starts=torch.tensor([n - m for n, m in zip(lens, new)], dtype=torch.int32, device=dev),
+                 total=total, max_new=max(new), max_len=max(lens), n_rep=hq // hkv, scale=d ** -0.5, dtype=dtype)
+    if case["op"] == "write":  # K and V as slices of one fused projection's output
+        qkv = torch.empty(total, (hq + 2 * hkv) * d, dtype=dtype, device=dev)
+        kv = qkv[:, hq * d:].unflatten(1, (2, hkv, d))
+        kv[:, 0] = _rows(gen, total, hkv, d, dev)
+        kv[:, 1] = _rows(gen, total, hkv, d, dev)
+        state.update(k_new=kv[:, 0], v_new=kv[:, 1])
+    elif case["op"] != "readback":
+        state["q"] = torch.randn(total, hq, d, generator=gen, device=dev).to(dtype)
+    if case["op"] == "decode":
+        state["lse"] = torch.empty(B, hq, dtype=torch.float32, device=dev)
+    return state
+
+
+# ---- the plain forms ---------------------------------------------------------
+def _quantise(x):
+    """float rows [..., d] -> e4m3 codes, and the scales' bytes (exponent + 127; 255 with NaN codes for a row that
+    is not finite)."""
+    x = x.float()
+    amax = x.abs().amax(-1)
+    m, ex = torch.frexp(amax)  # amax = m * 2^ex, m in [0.5, 1)
+    e = (ex - 9 + (m > 0.875)).clamp(-127, 120)
+    e = torch.where(amax == 0, torch.full_like(e, -127), e)
+    good = torch.isfinite(amax)
+    codes = (x * torch.exp2(-e.double()).float().unsqueeze(-1)).masked_fill(~good.unsqueeze(-1), float("nan"))
+    codes = codes.to(torch.float8_e4m3fn)
+    return codes, (e + 127).masked_fill(~good, 255).to(torch.uint8)
+
+
+def _scale_of(byte):
+    return torch.exp2(byte.double() - 127).float().masked_fill(byte == 255, float("nan"))
+
+
+def _gathered(codes, scales, pages):
+    """The values of the pages [...], as [..., 16, hkv, d] in 32 bits."""
+    c = codes.view(torch.uint8)[pages].view(torch.float8_e4m3fn).float()
+    return c.mul_(_scale_of(scales[pages]).transpose(-1, -2).unsqueeze(-1))
+
+
+def _of_tokens(s, codes, scales, request, position):
+    """The values of single cached tokens, [tokens, hkv, d] in 32 bits."""
+    page, slot = s["table"].long()[request, position // PAGE], position % PAGE
+    c = codes.view(torch.uint8)[page, slot].view(torch.float8_e4m3fn).float()
+    return c.mul_(_scale_of(scales[page, :, slot]).unsqueeze(-1))
+
+
+def _new_tokens(s):
+    """Request and position of each of the packed new tokens."""
+    i = torch.arange(s["total"], device=s["cu"].device)
+    request = torch.searchsorted(s["cu"][1:].long(), i, right=True)
+    return request, s["starts"].long()[request] + i - s["cu"].long()[request]
+
+
+def _plain_write(s):
+    request, position = _new_tokens(s)
+    page, slot = s["table"].long()[request, position // PAGE], position % PAGE
+    for x, codes, scales in ((s["k_new"], s["k_codes"], s["k_scales"]), (s["v_new"], s["v_codes"], s["v_scales"])):
+        c, e = _quantise(x)
+        codes.view(torch.uint8)[page, slot] = c.view(torch.uint8)
+        scales[page, :, slot] = e
+    return _plain_readback(s)
+
+
+def _plain_readback(s):
+    request, position = _new_tokens(s)
+    return tuple(_of_tokens(s, s[c], s[e], request, position).to(s["dtype"])
+                 for c, e in (("k_codes", "k_scales"), ("v_codes", "v_scales")))
+
+
+def _plain_attention(s, q, lens, visible):
+    """q [B, n, hq, d] in 32 bits, visible [B, n]: each query sees the first `visible` tokens of its request.
+    -> out [B, n, hq, d] (0 where nothing is seen), the row sums' logarithm."""
+    B, n, hq, d = q.shape
+    pages = s["table"].long()
+    k = _gathered(s["k_codes"], s["k_scales"], pages).flatten(1, 2).transpose(1, 2)  # [B, hkv, T, d]
+    hkv, T = k.shape[1], k.shape[2]
+    qg = q.transpose(1, 2).reshape(B, hkv, -1, d)  # rows (head of the group, query)
+    scores = torch.matmul(qg, k.transpose(2, 3)).mul_(s["scale"]).view(B, hkv, hq // hkv, n, T)
+    del k
+    t = torch.arange(T, device=q.device)
+    scores.masked_fill_(t >= visible[:, None, None, :, None], float("-inf"))
+    top = scores.amax(-1, keepdim=True)
+    top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+    w = scores.sub_(top).exp_()
+    total = w.sum(-1, keepdim=True)
+    v = _gathered(s["v_codes"], s["v_scales"], pages).flatten(1, 2).transpose(1, 2)
+    v = v * (t < lens[:, None])[:, None, :, None]  # what lies behind a request's last token is never read
+    out = torch.matmul(w.view(B, hkv, -1, T), v).view(B, hkv, hq // hkv, n, d)
+    out = torch.where(total > 0, out / total, torch.zeros_like(out))
+    lse = (top + total.log()).squeeze(-1)
+    return out.reshape(B, hq, n, d).transpose(1, 2), lse.reshape(B, hq, n)
+
+
+def _plain_decode(s):
+    lens = s["lens"].long()
+    out, lse = _plain_attention(s, s["q"].float().unsqueeze(1), lens, lens.unsqueeze(1))
+    return out.squeeze(1).to(s["dtype"]), lse.squeeze(-1)
+
+
+def _plain_chunk(s):
+    request, position = _new_tokens(s)
+    row = position - s["starts"].long()[request]
+    lens, B = s["lens"].long(), s["table"].shape[0]
+    q = torch.zeros(B, s["max_new"], *s["q"].shape[1:], dtype=torch.float32, device=s["q"].device)
+    q[request, row] = s["q"].float()
+    visible = s["starts"].long()[:, None] + torch.arange(s["max_new"], device=q.device) + 1
+    out, _ = _plain_attention(s, q, lens, visible)
+    return out[request, row].to(s["dtype"])
+
+
+# ---- one pass ----------------------------------------------------------------
+def run(state):
+    s, op = state, state["case"]["op"]
+    if own:
+        from unifiedkv_b200 import kv_quant
+        kv = kv_quant.QuantPagedKV(s["k_codes"], s["v_codes"], s["k_scales"], s["v_scales"])
+        if op == "write":
+            kv_quant.quantize_append(kv, s["k_new"], s["v_new"], s["table"], s["lens"], cu_seqlens_q=s["cu"])
+        if op in ("write", "readback"):
+            return kv_quant.dequantize_pages(kv, s["table"], s["cu"], s["total"], dtype=s["dtype"],
+                                             starts=s["starts"])
+        if op == "decode":
+            out = kv_quant.page16_decode_attention_q8(s["q"], kv, s["table"], s["lens"],
+                                                      softmax_scale=s["scale"], n_rep=s["n_rep"], lse_out=s["lse"])
+            return out, s["lse"]
+        return kv_quant.paged_chunk_prefill_q8(s["q"], kv, s["table"], softmax_scale=s["scale"],
+                                               n_rep=s["n_rep"], cu_seqlens_q=s["cu"], seqlens_k=s["lens"],
+                                               max_seqlen_q=s["max_new"])
+    return {"write": _plain_write, "readback": _plain_readback, "decode": _plain_decode, "chunk": _plain_chunk}[op](s)
+
+
+def work(case):
+    lens, new = _lengths(case)
+    hq, hkv, d = case["hq"], case["hkv"], case["d"]
+    elem = DTYPES[case["dtype"]].itemsize
+    total, row = sum(new), 2 * hkv * (d + 1)  # a token's codes and scales, K and V
+    dense = 2 * total * hkv * d * elem
+    if case["op"] == "readback":
+        return {"bytes": total * row + dense, "flops": 2 * total * hkv * d}
+    if case["op"] == "write":  # read K and V, write the cache, write what it now holds
+        return {"bytes": 2 * dense + total * row, "flops": 8 * total * hkv * d}
+    tables = 4 * sum(_pages(n) for n in lens)
+    pairs = sum(m * (n - m) + m * (m + 1) // 2 for n, m in zip(lens, new))
+    return {"bytes": sum(n for n, m in zip(lens, new) if m) * row + 2 * total * hq * d * elem + tables,
+            "flops": 4 * hq * d * pairs}
+
+
+# ---- from the definition, in 64 bits -------------------------------------------
+def _pow2(e):
+    """2^e of whole numbers, exactly: the exponent field of a 64-bit number."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
+def _exact_values(codes_u8, byte):
+    """e4m3 codes by their bit fields, times 2^(byte - 127)."""
+    c = codes_u8.to(torch.int64)
+    field, frac = (c >> 3) & 15, (c & 7).double()
+    mag = torch.where(field == 0, frac * 2.0 ** -9, (8 + frac) * _pow2(field - 10))
+    val = torch.where(c >= 128, -mag, mag)
+    return val * _pow2(byte.to(torch.int64) - 127).unsqueeze(-1)
+
+
+def _exact_round_trip(x):
+    """Rows [n, hkv, d] -> the values the cache holds for them."""
+    x = x.double()
+    amax = x.abs().amax(-1, keepdim=True)
+    e = torch.ceil(torch.log2(amax / E4M3_MAX)).clamp(-140, 140).to(torch.int64)
+    e = torch.where(amax <= E4M3_MAX * _pow2(e - 1), e - 1, e)  # a logarithm may be off by one at a border
+    e = torch.where(amax > E4M3_MAX * _pow2(e), e + 1, e).clamp(-127, 120)
+    y = x / _pow2(e)
+    _, octave = torch.frexp(y.abs().clamp_min(2.0 ** -6))  # |y| in [2^(octave-1), 2^octave)
+    step = _pow2(octave.to(torch.int64) - 4)
+    return torch.round(y / step) * step * _pow2(e)  # torch.round: halves to even
+
+
+def _exact_request(s, b, n, codes, scales):
+    pages = s["table"][b, :_pages(n)].long()
+    values = _exact_values(codes.view(torch.uint8)[pages], scales[pages].transpose(1, 2))
+    return values.reshape(-1, *values.shape[2:])[:n]
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    lens, new = _lengths(case)
+    if case["op"] == "write":
+        return _exact_round_trip(s["k_new"]), _exact_round_trip(s["v_new"])
+    if case["op"] == "readback":
+        got = [[_exact_request(s, b, n, s[c], s[e])[n - m:] for b, (n, m) in enumerate(zip(lens, new))]
+               for c, e in (("k_codes", "k_scales"), ("v_codes", "v_scales"))]
+        return tuple(torch.cat(g) for g in got)
+    if case["hq"] * case["d"] * sum(n * m for n, m in zip(lens, new)) > 4e11:
+        return None
+    q, out, lse, at = s["q"].double(), [], [], 0
+    for b, (n, m) in enumerate(zip(lens, new)):
+        k = _exact_request(s, b, n, s["k_codes"], s["k_scales"])
+        v = _exact_request(s, b, n, s["v_codes"], s["v_scales"])
+        qb = q[at:at + m]
+        at += m
+        o = torch.empty_like(qb)
+        hidden = torch.arange(n, device=q.device) > torch.arange(n - m, n, device=q.device)[:, None]
+        for h in range(case["hq"]):
+            g = h // s["n_rep"]
+            x = (qb[:, h] @ k[:, g].T * s["scale"]).masked_fill(hidden, -math.inf)
+            o[:, h] = torch.softmax(x, -1) @ v[:, g]
+            lse.append(torch.logsumexp(x, -1))
+        out.append(o)
+    out = torch.cat(out)
+    if case["op"] == "decode":
+        return out, torch.cat(lse).view(len(lens), case["hq"])
+    return out
