@@ -3,8 +3,8 @@
 The cache holds the K and V row of every (token, KV head) as head_dim e4m3 codes and one
 power-of-two scale (an e8m0 byte: exponent + 127), in pages of 16 tokens:
 codes [pages, 16, kv_heads, head_dim], scales [pages, kv_heads, 16].  The scale is the smallest
-2^e with max|row| <= 448 * 2^e (e >= -127), so a stored value is code * 2^e and dividing by the
-scale is exact: the codes do not depend on the precision they are computed in.
+2^e with max|row| <= 448 * 2^e (-127 <= e <= 119), so a stored value is code * 2^e and dividing by
+the scale is exact: the codes do not depend on the precision they are computed in.
 
 Four operators ("op" of a case):
   write     the new tokens of every request quantised into its pages, then read back
@@ -175,11 +175,11 @@ def _quantise(x):
     x = x.float()
     amax = x.abs().amax(-1)
     m, ex = torch.frexp(amax)  # amax = m * 2^ex, m in [0.5, 1)
-    e = (ex - 9 + (m > 0.875)).clamp(-127, 120)
+    e = (ex - 9 + (m > 0.875)).clamp(-127, 119)
     e = torch.where(amax == 0, torch.full_like(e, -127), e)
     good = torch.isfinite(amax)
-    codes = (x * torch.exp2(-e.double()).float().unsqueeze(-1)).masked_fill(~good.unsqueeze(-1), float("nan"))
-    codes = codes.to(torch.float8_e4m3fn)
+    y = (x * torch.exp2(-e.double()).float().unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX)
+    codes = y.masked_fill(~good.unsqueeze(-1), float("nan")).to(torch.float8_e4m3fn)
     return codes, (e + 127).masked_fill(~good, 255).to(torch.uint8)
 
 
@@ -322,8 +322,8 @@ def _exact_round_trip(x):
     amax = x.abs().amax(-1, keepdim=True)
     e = torch.ceil(torch.log2(amax / E4M3_MAX)).clamp(-140, 140).to(torch.int64)
     e = torch.where(amax <= E4M3_MAX * _pow2(e - 1), e - 1, e)  # a logarithm may be off by one at a border
-    e = torch.where(amax > E4M3_MAX * _pow2(e), e + 1, e).clamp(-127, 120)
-    y = x / _pow2(e)
+    e = torch.where(amax > E4M3_MAX * _pow2(e), e + 1, e).clamp(-127, 119)
+    y = (x / _pow2(e)).clamp(-E4M3_MAX, E4M3_MAX)
     _, octave = torch.frexp(y.abs().clamp_min(2.0 ** -6))  # |y| in [2^(octave-1), 2^octave)
     step = _pow2(octave.to(torch.int64) - 4)
     return torch.round(y / step) * step * _pow2(e)  # torch.round: halves to even
