@@ -386,6 +386,64 @@ BPKV_API int bpkv_page_gather(const void* pool, const int32_t* page_ids, int n_p
 BPKV_API int bpkv_page_scatter(const void* packed, const int32_t* page_ids, int n_pages, void* pool,
                       int64_t page_elems, int64_t page_stride, int dtype, void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * 8-bit paged KV cache (no counterpart in the reference, whose pool is 16-bit,
+ * core/pool.py:20-71).  A row (token, KV head) of K or V is head_dim e4m3 codes
+ * and one scale byte: value = code * 2^(byte - 127), with the smallest exponent
+ * in [-127, 119] for which max|row| <= 448 * 2^e; a row with an infinity or a
+ * NaN is stored as NaN codes with byte 255.  One layer:
+ *   codes  [num_pages][16][num_kv_heads][head_dim], a page dense, page_stride bytes apart
+ *   scales [num_pages][num_kv_heads][16],           a page dense, scale_stride bytes apart
+ * K and V share the strides; both are multiples of 16 and every base is 16-byte
+ * aligned.  head_dim is 64, 128 or 256.  A block-table entry outside
+ * [0, num_pages) is a page that is not there: never read or written.
+ * ------------------------------------------------------------------------ */
+
+/* Quantise new tokens into their pages.  k_new/v_new: rows [total_q,
+ * num_kv_heads, head_dim] of dtype (F32, F16, BF16) with token and head strides
+ * of multiples of 16 bytes.  seqlens_k [batch]: a request's tokens with the new
+ * ones; cu_seqlens_q [batch + 1] bounds its new rows (NULL: one row per request,
+ * total_q == batch).  Row i of a request's n new ones goes to position
+ * seqlens_k - n + i; rows without a page, or outside every sequence, are skipped. */
+BPKV_API int bpkv_q8_append(const void* k_new, const void* v_new, void* k_codes, void* v_codes,
+                      uint8_t* k_scales, uint8_t* v_scales, const int32_t* block_table,
+                      const int32_t* cu_seqlens_q, const int32_t* seqlens_k, int batch, int total_q,
+                      int num_kv_heads, int head_dim, int max_blocks, int num_pages,
+                      int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                      int64_t page_stride, int64_t scale_stride, int64_t bt_stride_b, int dtype,
+                      void* stream);
+
+/* Read ranges of tokens back as dense rows: row cu_seqlens[b] + j of k_out/v_out
+ * [total, num_kv_heads, head_dim] (dtype, strides out_stride_t/out_stride_h) is
+ * token starts[b] + j of request b (starts NULL: 0).  Tokens without a page read
+ * as zeros; rows outside every range keep what they held. */
+BPKV_API int bpkv_q8_dequantize(const void* k_codes, const void* v_codes, const uint8_t* k_scales,
+                      const uint8_t* v_scales, const int32_t* block_table, const int32_t* cu_seqlens,
+                      const int32_t* starts, void* k_out, void* v_out, int batch, int total,
+                      int num_kv_heads, int head_dim, int max_blocks, int num_pages,
+                      int64_t page_stride, int64_t scale_stride, int64_t bt_stride_b,
+                      int64_t out_stride_t, int64_t out_stride_h, int dtype, void* stream);
+
+/* Attention over 8-bit pages: the 8-bit forms of bpkv_page16_decode (cu_seqlens_q
+ * NULL, max_seqlen_q 1: row b of q is request b's) and bpkv_paged_prefill.
+ * q: [total_q, num_q_heads, head_dim] (F16 or BF16), token and head strides of
+ * multiples of 16 bytes; out: the same, contiguous; lse_out: fp32 [total_q,
+ * num_q_heads] natural-log sum-exp, or NULL.  Query i of a request's n sees its
+ * tokens t <= seqlens_k - n + i (all of them when causal is 0) that have a page.
+ * A query that sees none gives zeros, or NaN with empty_nan, and lse -inf.
+ * Chunks longer than max_seqlen_q are cut there.
+ * workspace: bpkv_q8_attention_workspace_size() bytes (may be 0). */
+BPKV_API size_t bpkv_q8_attention_workspace_size(int batch, int num_q_heads, int num_kv_heads,
+                      int head_dim, int max_seqlen_q);
+BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, const void* v_codes,
+                      const uint8_t* k_scales, const uint8_t* v_scales, const int32_t* block_table,
+                      const int32_t* cu_seqlens_q, const int32_t* seqlens_k, void* out, float* lse_out,
+                      int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_blocks,
+                      int num_pages, int max_seqlen_q, int64_t q_stride_t, int64_t q_stride_h,
+                      int64_t page_stride, int64_t scale_stride, int64_t bt_stride_b,
+                      float softmax_scale, int causal, int empty_nan, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,8 @@ def paged_chunk_prefill(q_chunk: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     s = k_cache.stride()
     if s[3] != 1 or s[2] != d or s[1] != h_kv * d or v_cache.stride() != k_cache.stride():
         raise RuntimeError("prefill_shape_unsupported:cache_layout")
+    if k_cache.dtype != q_chunk.dtype or v_cache.dtype != q_chunk.dtype:
+        raise RuntimeError("prefill_shape_unsupported:dtype_mismatch")
     dev = q_chunk.device
     B = int(block_table.shape[0])
     if cu_seqlens_q is None or seqlens_k is None:
@@ -71,6 +73,8 @@ def append_chunk_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, k_chunk: torch
     n = int(k_chunk.shape[1])
     if n == 0:
         return
+    if k_cache.element_size() == 1:  # 8-bit pages need their scales (kv_quant.quantize_append)
+        raise RuntimeError("prefill_shape_unsupported:dtype_mismatch")
     first = past_len // 16
     last = (past_len + n - 1) // 16
     off = past_len - first * 16

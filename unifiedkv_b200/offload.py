@@ -32,6 +32,7 @@ from .pool import PagedKVPool
 
 class AsyncOffloadManager:
     def __init__(self, pool: PagedKVPool, num_layers: int, host_slots: int = 0, staging_pages: int = 512):
+        _lib.dtype_code(pool.dtype)  # refuses a pool whose pages are more than one tensor (8-bit codes with scales)
         self.pool = pool
         self.num_layers = int(num_layers)
         self.lock = threading.Lock()

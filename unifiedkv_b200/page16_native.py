@@ -170,6 +170,8 @@ def decode_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tenso
         raise RuntimeError("decode_append_shape_unsupported:shape")
     if not (_page_view_ok(k_cache, h_kv, d) and _page_view_ok(v_cache, h_kv, d)) or k_cache.stride(0) != v_cache.stride(0):
         raise RuntimeError("decode_append_shape_unsupported:cache_layout")
+    if not (k_new.dtype == v_new.dtype == k_cache.dtype == v_cache.dtype):
+        raise RuntimeError("decode_append_shape_unsupported:dtype_mismatch")
     k_new = k_new.contiguous()
     v_new = v_new.contiguous()
     bt = block_table.to(torch.int32).contiguous()
