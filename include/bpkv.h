@@ -433,13 +433,14 @@ BPKV_API int bpkv_q8_dequantize(const void* k_codes, const void* v_codes, const 
  * A query that sees none gives zeros, or NaN with empty_nan, and lse -inf.
  * Chunks longer than max_seqlen_q are cut there.
  * workspace: bpkv_q8_attention_workspace_size() bytes (may be 0). */
-BPKV_API size_t bpkv_q8_attention_workspace_size(int batch, int num_q_heads, int num_kv_heads,
-                      int head_dim, int max_seqlen_q);
+BPKV_API size_t bpkv_q8_attention_workspace_size(int batch, int total_q, int num_q_heads,
+                      int num_kv_heads, int head_dim, int max_blocks, int max_seqlen_q,
+                      float softmax_scale);
 BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, const void* v_codes,
                       const uint8_t* k_scales, const uint8_t* v_scales, const int32_t* block_table,
                       const int32_t* cu_seqlens_q, const int32_t* seqlens_k, void* out, float* lse_out,
-                      int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_blocks,
-                      int num_pages, int max_seqlen_q, int64_t q_stride_t, int64_t q_stride_h,
+                      int batch, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                      int max_blocks, int num_pages, int max_seqlen_q, int64_t q_stride_t, int64_t q_stride_h,
                       int64_t page_stride, int64_t scale_stride, int64_t bt_stride_b,
                       float softmax_scale, int causal, int empty_nan, int dtype, void* workspace,
                       size_t workspace_bytes, void* stream);

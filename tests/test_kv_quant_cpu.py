@@ -174,18 +174,19 @@ def test_library_checks_without_a_gpu():
         assert append(**kw) == _lib.BPKV_ERR_SHAPE and token in _lib.last_error(), (kw, _lib.last_error())
     assert append(total=0, batch=0) == 0  # nothing to do: no launch
 
-    def attend(hq=4, h=2, d=64, batch=1, max_q=1, cu=None, dtype=2, q=a, ws=None, ws_bytes=0, qst=256, max_blocks=1):
-        return L.bpkv_q8_attention(q, a, a, a, a, a, cu, a, a, None, batch, hq, h, d, max_blocks, 3, max_q, qst, 64, 2048, 32, 1,
+    def attend(hq=4, h=2, d=64, batch=1, total=1, max_q=1, cu=None, dtype=2, q=a, ws=None, ws_bytes=0, qst=256, max_blocks=1):
+        return L.bpkv_q8_attention(q, a, a, a, a, a, cu, a, a, None, batch, total, hq, h, d, max_blocks, 3, max_q, qst, 64, 2048, 32, 1,
                                    0.1, 1, 0, dtype, ws, ws_bytes, None)
 
-    for kw, token in ((dict(hq=3), "gqa"), (dict(d=80), "head_dim_80"), (dict(dtype=0), "dtype_0"), (dict(max_q=2), "max_seqlen_q"),
+    for kw, token in ((dict(hq=3), "gqa"), (dict(d=80), "head_dim_80"), (dict(dtype=0), "dtype_0"), (dict(max_q=2), "max_seqlen_q"), (dict(total=2), "max_seqlen_q"),
                       (dict(q=None), "null_pointer"), (dict(q=a + 4), "alignment"), (dict(qst=100), "alignment"),
                       (dict(max_blocks=1 << 27), "max_blocks")):
         assert attend(**kw) == _lib.BPKV_ERR_SHAPE and token in _lib.last_error(), (kw, _lib.last_error())
     assert attend() == _lib.BPKV_ERR_WORKSPACE and "workspace" in _lib.last_error()
-    assert attend(batch=0) == 0
+    assert attend(batch=0, total=0) == 0
     need = L.bpkv_q8_attention_workspace_size
-    assert need(1, 3, 2, 64, 1) == 0 and need(1, 4, 2, 96, 1) == 0 and need(4, 32, 8, 128, 1) > 0
+    assert need(1, 1, 3, 2, 64, 9, 1, 0.1) == 0 and need(1, 1, 4, 2, 96, 9, 1, 0.1) == 0
+    assert need(4, 4, 32, 8, 128, 9, 1, 0.1) > 0
 
 
 def test_pool_bookkeeping_and_layout():

@@ -12,8 +12,15 @@ Bounds of an output element, with A = sum p |v| / sum p:
     numerator and denominator each move by ln2 dx + 2^-22, the output by twice that of A;
   * sums of n weights in fp32 lose at most a further 2^-24 per addition on a chain; the
     longest chain of one lane is n / 16 pages long, merged pairwise: n 2^-28 A at most twice;
-  * q is taken to fp16 after scaling its row to [2^14, 2^15): elements below 2^-29 of the
-    row's largest lose at most 2^-40 of that largest, inside the bound on dx.
+  * fp16 ends at 2^-25 (half a step of its subnormals).  A weight is held in units of 2^-11
+    of a reference at or below the row's largest weight, so it is off by 2^-36 of that at
+    most; where the value's scale is in the weight too (units of 2^-12 of the largest scale,
+    codes up to 448, that scale at most vmax / 224) by 2^-37 448 / 224 vmax = 2^-36 vmax; a
+    value held as 2^-6 of the largest scale and up by 2^-25 2^-6 / 224 vmax < 2^-38 vmax: n
+    tokens move the output by (n + 1) 2^-36 vmax, vmax the request's largest |v|;
+  * likewise keys relative to the largest scale of a tile are off by 2^-25 kmax / 224, and q
+    after scaling its row to [2^14, 2^15) by 2^-25 2^-14 of the row's largest: d products
+    move x by d 2^-32 log2(e) scale qmax kmax at most.
 The log-sum-exp moves by ln2 dx + 2^-22, and is rounded to fp32 a few times.
 """
 import math
@@ -85,10 +92,18 @@ def _check(got, lse, q, kv, bt, lens, new, scale, causal=True, empty=0.0, weight
             assert np.isnan(o[none]).all()
         else:
             assert (o[none] == empty).all()
-        dx = (d + 8) * 2.0 ** -24 * size
+        qmax = np.abs(np.where(np.isfinite(qn[at - m:at]), qn[at - m:at], 0)).max(-1)
+        kmax, vmax = (np.nanmax(np.abs(x), initial=0.0) for x in (k, v))
+        dx = (d + 8) * 2.0 ** -24 * size + d * 2.0 ** -32 * scale * qmax * kmax
         move = dx + 2.0 ** -21 + n * 2.0 ** -27
-        tol = half * np.abs(ref) + (weight + 2 * move)[..., None] * mean_abs * (1 + half) + tiny
-        bad = ~none[..., None] & ~(np.abs(o - ref) <= tol)
+        floor = (n + 1) * 2.0 ** -36 * vmax
+        tol = half * np.abs(ref) + ((weight + 2 * move)[..., None] * mean_abs + floor) * (1 + half) + tiny
+        with np.errstate(invalid="ignore"):
+            near = np.abs(o - ref) <= tol
+        # what lies half a step or more above the type's largest number rounds to an infinity
+        top = torch.finfo(got.dtype).max * (1 + half / 2)
+        near |= (np.abs(ref) + tol >= top) & np.isinf(o) & (np.sign(o) == np.sign(ref))
+        bad = ~none[..., None] & ~near
         assert not bad.any(), (b, n, m, np.argwhere(bad)[:5], o[bad][:5], ref[bad][:5], tol[bad][:5])
         if l is not None:
             assert np.isneginf(l[none]).all()
@@ -545,3 +560,103 @@ def test_no_synchronisation_and_no_empty_launch(cuda):
     finally:
         torch.cuda.set_sync_debug_mode("default")
     assert k.shape == (0, 2, 64) and v.shape == (0, 2, 64) and out.shape == (0, 2, 64)
+
+
+# ---- the tensor-core chunk kernel --------------------------------------------------
+def _chunk(cuda, q, kv, bt, lens, new, n_rep, scale, causal=True):
+    from unifiedkv_b200.kv_quant import paged_chunk_prefill_q8
+    lse = torch.full(q.shape[:2], 9.0, device=cuda)
+    out = paged_chunk_prefill_q8(q, kv, bt, softmax_scale=scale, n_rep=n_rep, causal=causal, cu_seqlens_q=_cu(cuda, new),
+                                 seqlens_k=_i32(cuda, lens), max_seqlen_q=max(new), lse_out=lse)
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,lens", [
+    ([40], [5000]),                 # 120 rows: alternating groups, the tokens split over CTAs
+    ([100, 90], [130, 3000]),       # two row tiles, one of them partly empty
+    ([43, 1, 20], [43, 4000, 129]),
+    ([171], [4096]),                # 513 rows: a tile of one row
+])
+def test_long_caches(cuda, dtype, d, new, lens):
+    n_pages = sum(-(-n // 16) for n in lens) + 2
+    kv = _fill(cuda, n_pages, 1, d, seed=d + sum(new), spread=1.0)
+    bt = _table(cuda, lens, n_pages, seed=50)
+    g = torch.Generator(device=cuda).manual_seed(8)
+    q = torch.randn(sum(new), 3, d, generator=g, device=cuda).to(DT[dtype])
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, 3, d ** -0.5)
+    again, _ = _chunk(cuda, q, kv, bt, lens, new, 3, d ** -0.5)
+    assert torch.equal(out, again)
+    _check(out, lse, q, kv, bt, lens, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("k_spread,v_spread", [(0.0, 0.0), (1.0, 4.0)])
+def test_chunk_with_scales_far_apart(cuda, dtype, k_spread, v_spread):
+    """Scales that move the values' reference from tile to tile, and rows of q of very unequal norm."""
+    lens, new = [900, 300], [70, 30]
+    kv = _fill(cuda, 90, 1, 128, seed=51, spread=k_spread, v_spread=v_spread)
+    bt = _table(cuda, lens, 90, seed=52)
+    table = bt.cpu().numpy()
+    kv.v_scales[int(table[0, 40])] += 30  # one page's values 2^30 above the rest: the reference jumps late
+    q = torch.randn(100, 2, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(9)).to(DT[dtype])
+    q[::7] = 0
+    q[1::7] *= 8
+    q[2::7] *= 2.0 ** -12
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, 2, 0.05)
+    _check(out, lse, q, kv, bt, lens, new, 0.05)
+
+
+def test_chunk_over_pages_that_are_not_there(cuda):
+    lens, new = [600, 150, 64], [64, 50, 50]
+    kv = _fill(cuda, 60, 2, 128, seed=53)
+    bt = _table(cuda, lens, 60, seed=54)
+    bt[0, 0] = -1
+    bt[0, 9:30] = 60
+    bt[0, 36] = -5
+    bt[2] = -1  # nothing of request 2 is there
+    q = torch.randn(sum(new), 4, 128, device=cuda).bfloat16()
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, 2, 0.1)
+    _check(out, lse, q, kv, bt, lens, new, 0.1)
+
+
+@pytest.mark.parametrize("hq,h_kv,d,new", [(4, 2, 128, 60), (4, 2, 64, 3), (4, 1, 256, 20)])
+def test_negative_and_zero_softmax_scales(cuda, hq, h_kv, d, new):
+    lens = [new + 100]
+    kv = _fill(cuda, 20, h_kv, d, seed=55)
+    bt = _table(cuda, lens, 20, seed=56)
+    q = torch.randn(new, hq, d, device=cuda).bfloat16()
+    for scale in (-0.1, 0.0):
+        out, lse = _chunk(cuda, q, kv, bt, lens, [new], hq // h_kv, scale)
+        dx = max(abs(scale), 1e-30)
+        assert torch.isfinite(lse).all()
+        kc, vc, ks, vs = _np(kv)
+        k, there = oracle.request_rows(kc, ks, bt.cpu().numpy()[0], lens[0])
+        v, _ = oracle.request_rows(vc, vs, bt.cpu().numpy()[0], lens[0])
+        ref, ref_lse, mean_abs, size = oracle.attention(q.double().cpu().numpy(), k, v, there, new, scale)
+        move = (d + 8) * 2.0 ** -24 * np.abs(size) + 2.0 ** -21 + lens[0] * 2.0 ** -27
+        tol = 2.0 ** -8 * np.abs(ref) + (2.0 ** -11 + 2 * move)[..., None] * mean_abs * (1 + 2.0 ** -8)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all(), (scale, dx)
+
+
+def test_chunks_of_values_that_are_not_finite(cuda):
+    """NaN keys and values in several tiles, rows of q that are not finite: only who sees them is NaN."""
+    lens, new = [700], [150]
+    kv = _fill(cuda, 50, 1, 128, seed=57)
+    bt = _table(cuda, lens, 50, seed=58)
+    table = bt.cpu().numpy()[0]
+    q = torch.randn(150, 2, 128, device=cuda).bfloat16()
+    clean, _ = _chunk(cuda, q, kv, bt, lens, new, 2, 0.1)
+    for pos, (codes, scales) in ((600, (kv.v_codes, kv.v_scales)), (640, (kv.k_codes, kv.k_scales))):
+        codes.view(torch.uint8)[int(table[pos // 16]), pos % 16] = 0x7F
+        scales[int(table[pos // 16]), :, pos % 16] = 255
+    q[3, 1, 5] = float("inf")
+    q[4, 0, 7] = float("nan")
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, 2, 0.1)
+    first = 600 - 550  # query i sees tokens up to 550 + i
+    assert torch.isnan(out[first:]).all() and torch.isnan(out[3, 1]).all() and torch.isnan(out[4, 0]).all()
+    keep = torch.ones(150, 2, dtype=torch.bool, device=cuda)
+    keep[first:] = False
+    keep[3, 1] = keep[4, 0] = False
+    assert torch.equal(out[keep], clean[keep])

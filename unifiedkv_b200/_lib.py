@@ -78,8 +78,8 @@ SIGNATURES = {
                                      _c_f, _c_int, _c_int, _c_p]),
     "bpkv_q8_append": (_c_int, [_c_p] * 9 + [_c_int] * 6 + [_c_i64] * 7 + [_c_int, _c_p]),
     "bpkv_q8_dequantize": (_c_int, [_c_p] * 9 + [_c_int] * 6 + [_c_i64] * 5 + [_c_int, _c_p]),
-    "bpkv_q8_attention_workspace_size": (_c_sz, [_c_int, _c_int, _c_int, _c_int, _c_int]),
-    "bpkv_q8_attention": (_c_int, [_c_p] * 10 + [_c_int] * 7 + [_c_i64] * 5 +
+    "bpkv_q8_attention_workspace_size": (_c_sz, [_c_int] * 7 + [_c_f]),
+    "bpkv_q8_attention": (_c_int, [_c_p] * 10 + [_c_int] * 8 + [_c_i64] * 5 +
                           [_c_f, _c_int, _c_int, _c_int, _c_p, _c_sz, _c_p]),
     "bpkv_page_gather": (_c_int, [_c_p, _c_p, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_p]),
     "bpkv_page_scatter": (_c_int, [_c_p, _c_p, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_p]),

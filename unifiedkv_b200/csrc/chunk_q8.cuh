@@ -1,0 +1,29 @@
+// Launch parameters of the tensor-core chunk attention over 8-bit pages (chunk_q8_tc.cu).
+#pragma once
+
+#include "q8.cuh"
+
+namespace bpkv {
+
+struct ChunkQ8Params {
+  const void* q;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  const int32_t* bt;
+  const int32_t* cu_q;
+  const int32_t* lens;
+  void* out;
+  float* lse_out;
+  float* part_o;    // [parts][total_q * Hq][D]
+  float* part_lse;  // [parts][total_q * Hq]
+  int B, Hq, Hkv, n_rep, tiles, splits, parts, alt, causal, max_blocks, num_pages, total_q;
+  int64_t q_st, q_sh, page_stride, scale_stride, bt_sb;
+  float scale_log2;
+};
+
+// head_dim 64 or 128, softmax scale > 0.
+int chunk_q8_tc_launch(const ChunkQ8Params& p, int head_dim, int dtype, cudaStream_t st);
+
+}  // namespace bpkv

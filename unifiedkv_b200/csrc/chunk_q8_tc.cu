@@ -1,0 +1,731 @@
+// Attention of chunks of new tokens over 8-bit pages on the 5th-generation tensor
+// cores (tcgen05.mma, TMEM accumulators), sm_100a, head_dim 64 and 128.
+//
+// The mathematics is page16_q8.cu's; the rows of a request and KV head (query token
+// major, query head minor) are cut into tiles of 256 or 128.
+//
+// Design:
+//  * Bound.  A chunk does 4 * head_dim FLOP per (row, visible token): with hundreds of
+//    rows the tensor pipe and the exponentials bound it, not the pages' bytes.
+//  * Codes become fp16 operands on the way into shared memory.  Four converter warps
+//    bring 16-code pieces in by cp.async (one tile ahead, each thread its own), turn them
+//    into fp16 (cvt.rn.f16x2.e4m3x2 and one multiply per pair; e4m3 to bf16 takes five
+//    instructions a pair and made the converters the bound) and store them in the
+//    128-byte-swizzled layout of the UMMA descriptors, 128 tokens a tile, K and V each two
+//    tiles deep.  A key takes its scale relative to the tile's largest, which joins the
+//    softmax scale: one multiplier per tile.  A value takes its scale relative to a
+//    reference that follows the largest seen (64 above it stays in range; O is rescaled in
+//    the rare case that it moves).  Both are exact down to 2^-15 of the largest scale
+//    (values: 2^-21) and lose at most 2^-33 of the largest element below that.
+//  * q goes to fp16 with a power of two per row that brings the row into [2^14, 2^15):
+//    exact down to 2^-29 of the row's largest element, off by 2^-40 of it below.
+//  * Groups A and B of 8 softmax warps, 128 rows each, 2 threads per row.  The MMA warp
+//    issues PV_A S_A' PV_B S_B' so that one group's softmax runs under the other's
+//    MMAs.  With more than 128 rows A and B are two row tiles over the same K/V tiles;
+//    with fewer (alternating) both hold the same rows and take every other K/V tile.
+//  * Softmax: online in exp2, a reference maximum moved only when it lags by 2^4, one
+//    in 8 exponentials on the FMA pipe.  Weights go to TMEM as fp16 in units of 2^-11 (off
+//    by 2^-11 of each, against 2^-8 for a bf16 output; nothing above 2^-35 of the row's
+//    largest vanishes); fp16 outputs take them as a high and a low part.
+//  * Few rows over long caches: the K/V tiles of an item are cut into splits, each a
+//    CTA; these (and the two groups when alternating) leave fp32 (o, lse) parts that
+//    chunk_q8_merge_kernel joins.
+//  * Every wait is bounded (a poll count and 2 s); one that runs out ends in NaN rows.
+#include <type_traits>
+
+#include "chunk_q8.cuh"
+#include "f32x2.cuh"
+#include "tcgen05.cuh"
+
+namespace bpkv {
+
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kBM = 128, kBN = 128;   // rows of a group, tokens of a K/V tile
+constexpr int kRing = 2;              // K (and V) tiles in shared memory
+constexpr int kGroupWarps = 8;        // softmax warps of a group: warps 0 .. 15
+constexpr int kConvWarp = 16, kConvWarps = 4, kMmaWarp = 20;
+// Six warpgroups are launched with 80 registers a thread (61,440 in all) and share them out anew:
+// softmax 4 x 128 x 96, converters 128 x 64, MMA (and three idle warps) 128 x 32 = 61,440.
+constexpr int kThreads = 24 * 32;
+constexpr int kRegsSoftmax = 96, kRegsConv = 64, kRegsMma = 32;
+static_assert(128 * (4 * kRegsSoftmax + kRegsConv + kRegsMma) <= kThreads * 80, "register split");
+constexpr int kMaxPages = 2048;       // block-table entries staged in shared memory
+constexpr int kMaxRanked = 512;       // row tiles ordered longest first
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescale = 4.f, kWOff = 11.f;  // weights <= 2^4, held times 2^11
+constexpr int kVHead = 6;                      // values are held as code * 2^(byte - vref), byte <= vref + 6
+constexpr int kEmuStride = 8;
+
+// What the softmax warps need to know of a K/V tile, in a ring of 4: a slot is written with K(t + 4),
+// which needs S(t + 2) issued, which needs the softmax of tile t + 1 done.
+struct TileInfo {
+  float scale;       // softmax scale * log2(e) * 2^(largest key exponent)
+  int vref;          // reference byte of the values
+  uint32_t special;  // a token is missing (no page) or its value row is NaN
+  uint32_t missing[4];
+  uint32_t vnan[4];
+};
+constexpr int kInfo = 4;
+
+template <int D>
+struct Layout {
+  static constexpr int kDB = D / 64;
+  static constexpr int kQ = kDB * kBM * 128;   // bytes of a Q tile
+  static constexpr int kKV = kDB * kBN * 128;  // bytes of a K or V tile
+  static constexpr int kBars = 2 * kQ + 2 * kRing * kKV;
+  static constexpr int kInfoOff = kBars + 256;
+  static constexpr int kMx = kInfoOff + ((kInfo * static_cast<int>(sizeof(TileInfo)) + 15) / 16) * 16;
+  static constexpr int kL = kMx + 4 * 2 * 2 * 2 * kBM;  // after the row maxima, [group][2 buffers][half][row]
+  static constexpr int kQf = kL + 4 * 2 * 2 * kBM;      // after the row sums, [group][half][row]
+  static constexpr int kStage = kQf + 4 * 2 * kBM;      // after q's row factors, [group][row]
+  static constexpr int kPages = kStage + kBN * D;       // after the codes of one tile, on their way to a converter
+  static constexpr int kBytes = kPages + 4 * kMaxPages + 1024;  // + alignment
+};
+
+__device__ __forceinline__ uint32_t sw_off(int row, int chunk) {  // 16-byte chunk of a 128-byte swizzled row
+  return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// 2^e as an fp16 pair, e <= 15; 0 below the subnormals.
+__device__ __forceinline__ uint32_t f16_pow2(int e) {
+  const uint32_t x = e < -24 ? 0u : e < -14 ? 1u << (e + 24) : static_cast<uint32_t>(e + 15) << 10;
+  return x | x << 16;
+}
+
+struct RowTile {
+  int b, q0, n_q, n_rows, row0, kv_end;
+};
+__device__ __forceinline__ RowTile row_tile(const ChunkQ8Params& p, int i) {
+  RowTile r;
+  const int rows = p.alt ? kBM : 2 * kBM;
+  r.b = i / p.tiles;
+  r.row0 = (i % p.tiles) * rows;
+  r.q0 = __ldg(p.cu_q + r.b);
+  r.n_q = __ldg(p.cu_q + r.b + 1) - r.q0;
+  r.n_rows = r.n_q * p.n_rep;
+  const int len = __ldg(p.lens + r.b);
+  r.kv_end = 0;
+  if (r.row0 < r.n_rows) {
+    const int last = (min(r.row0 + rows, r.n_rows) - 1) / p.n_rep;
+    r.kv_end = min(max(p.causal ? len - r.n_q + last + 1 : len, 0), p.max_blocks * kPage);
+  }
+  return r;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_constant__ ChunkQ8Params p) {
+  using L = Layout<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t qs = smem_u32(smem), ks = qs + 2 * L::kQ, vs = ks + kRing * L::kKV;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  constexpr int kBarCount = 4 * kRing + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBarCount);
+  static_assert((kBarCount + 1) * 8 <= 256, "barrier area");
+  TileInfo* s_info = reinterpret_cast<TileInfo*>(smem + L::kInfoOff);
+  float* s_mx = reinterpret_cast<float*>(smem + L::kMx);
+  float* s_l = reinterpret_cast<float*>(smem + L::kL);
+  float* s_qf = reinterpret_cast<float*>(smem + L::kQf);
+  int* s_pages = reinterpret_cast<int*>(smem + L::kPages);
+
+  constexpr bool kTwoParts = std::is_same<T, __half>::value;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // ---- work item: (row tile, split, KV head), row tiles with most K/V tiles first ----
+  const int n_items = p.B * p.tiles;
+  const int hkv = static_cast<int>(blockIdx.x % p.Hkv);
+  const int split = static_cast<int>(blockIdx.x / p.Hkv) % p.splits;
+  int item = static_cast<int>(blockIdx.x / p.Hkv) / p.splits;
+  if (n_items <= kMaxRanked) {
+    __shared__ int s_item;
+    for (int i = tid; i < n_items; i += kThreads) s_pages[i] = row_tile(p, i).kv_end;
+    __syncthreads();
+    for (int i = tid; i < n_items; i += kThreads) {
+      const int wi = s_pages[i];
+      int rank = 0;
+      for (int j = 0; j < n_items; ++j) rank += (s_pages[j] > wi) || (s_pages[j] == wi && j < i);
+      if (rank == item) s_item = i;
+    }
+    __syncthreads();
+    item = s_item;
+    __syncthreads();  // s_pages is about to be filled
+  }
+  const RowTile rt = row_tile(p, item);
+  if (rt.row0 >= rt.n_rows) return;  // uniform across the CTA, before any barrier or TMEM use
+  const int all_tiles = (rt.kv_end + kBN - 1) / kBN;
+  const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
+  const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits) - tile0;
+  const int32_t* bt_row = p.bt + static_cast<int64_t>(rt.b) * p.bt_sb;
+
+  auto k_full = [&](int t) { return smem_u32(&bars[t % kRing]); };
+  auto v_full = [&](int t) { return smem_u32(&bars[kRing + t % kRing]); };
+  auto k_free = [&](int t) { return smem_u32(&bars[2 * kRing + t % kRing]); };
+  auto v_free = [&](int t) { return smem_u32(&bars[3 * kRing + t % kRing]); };
+  auto s_full = [&](int g) { return smem_u32(&bars[4 * kRing + g]); };
+  auto p_full = [&](int g) { return smem_u32(&bars[4 * kRing + 2 + g]); };
+  auto o_done = [&](int g) { return smem_u32(&bars[4 * kRing + 4 + g]); };
+
+  if (warp == 0) {
+    tc::tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tc::tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < kRing; ++i) {
+      tc::mbar_init(k_full(i), 32u * kConvWarps);
+      tc::mbar_init(v_full(i), 32u * kConvWarps);
+      tc::mbar_init(k_free(i), 1u);
+      tc::mbar_init(v_free(i), 1u);
+    }
+    for (int g = 0; g < 2; ++g) {
+      tc::mbar_init(s_full(g), 1u);
+      tc::mbar_init(p_full(g), 32u * kGroupWarps);
+      tc::mbar_init(o_done(g), 1u);
+    }
+    tc::fence_mbar_init();
+  }
+  const int page0 = tile0 * (kBN / kPage);
+  {
+    const int np = min(n_tiles * (kBN / kPage), kMaxPages);
+    for (int i = tid; i < np; i += kThreads) s_pages[i] = q8::page_of(bt_row, page0 + i, p.max_blocks, p.num_pages);
+  }
+  // ---- Q tiles -> shared memory as fp16, swizzled K-major; D / 8 neighbouring lanes share a row ----
+  {
+    constexpr int CPR = D / 8;
+    const int rows = p.alt ? kBM : 2 * kBM;
+    for (int e = tid; e < rows * CPR; e += kThreads) {  // kThreads and rows * CPR are multiples of 32
+      const int m = e / CPR, ch = e % CPR, r = rt.row0 + m;
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (r < rt.n_rows)
+        raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) +
+                                                   static_cast<int64_t>(rt.q0 + r / p.n_rep) * p.q_st +
+                                                   static_cast<int64_t>(hkv * p.n_rep + r % p.n_rep) * p.q_sh) + ch);
+      const T* x = reinterpret_cast<const T*>(&raw);
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(Elem<T>::to_f(x[i])) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 1; o < CPR; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      // rows of zeros, or not finite, stay as they are
+      int qe = static_cast<int>(amax >> 23) - 127 - 14;
+      qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
+      uint32_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = pack2<__half>(Elem<T>::to_f(x[2 * i]) * inv, Elem<T>::to_f(x[2 * i + 1]) * inv);
+      sts128(qs + (m / kBM) * L::kQ + (ch >> 3) * (kBM * 128) + sw_off(m % kBM, ch & 7), y[0], y[1], y[2], y[3]);
+      if (ch == 0) s_qf[m] = __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
+    }
+    tc::fence_proxy_async_smem();
+  }
+  tc::tc_fence_before();
+  __syncthreads();  // barriers initialised, TMEM address published, pages and Q staged
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto t_s = [&](int g) { return tmem + static_cast<uint32_t>(g * 256); };
+  auto t_o = [&](int g) { return tmem + static_cast<uint32_t>(g * 256 + 128); };
+  // group g's tile number k is K/V tile tile_at(g, k)
+  auto tile_at = [&](int g, int k) { return p.alt ? 2 * k + g : k; };
+
+  if (warp >= kConvWarp && warp < kMmaWarp) {
+    // =================== converters ===================
+    regs_dec<kRegsConv>();
+    // Thread ct handles 16-code piece ct % 4 of each 64-code block of rows ct / 4 + RS i: a quarter warp then
+    // stores whole swizzled rows of one block, without bank conflicts.
+    constexpr int RS = 8 * kConvWarps, N = kBN / RS, DB = L::kDB;
+    constexpr uint32_t kSlot = 32 * kConvWarps * 16;  // staging bytes of one piece of every thread
+    const int ct = tid - kConvWarp * 32;
+    const int ch = ct & 3, r0 = ct >> 2;
+    const int64_t in_page = static_cast<int64_t>(r0 & 15) * p.Hkv * D + static_cast<int64_t>(hkv) * D + ch * 16;
+    const uint8_t *kp = p.kc + in_page, *vp = p.vc + in_page;
+    const bool staged = n_tiles * (kBN / kPage) <= kMaxPages;
+    auto page_at = [&](int idx) {  // idx from page0
+      return staged || idx < kMaxPages ? s_pages[idx] : q8::page_of(bt_row, page0 + idx, p.max_blocks, p.num_pages);
+    };
+    const uint32_t stage = smem_u32(smem + L::kStage) + ct * 16;
+    // this thread's pieces of row r0 + RS i of a tile into its slots i of the staging area
+    auto fetch = [&](const uint8_t* base, int t, int i) {
+      const int page = page_at(t * (kBN / kPage) + RS / 16 * i + (r0 >> 4));
+      const bool ok = r0 + RS * i < rt.kv_end - (tile0 + t) * kBN && page >= 0;
+      const uint8_t* src = base + (ok ? page * p.page_stride : 0);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) cp_async16(stage + (i * DB + db) * kSlot, src + db * 64, ok);
+    };
+    auto byte_of_row = [&](uint32_t sc, int i) {
+      return static_cast<int>(__shfl_sync(0xffffffffu, sc, (r0 >> 2) + RS / 4 * i) >> ((r0 & 3) * 8) & 0xffu);
+    };
+    // 16 values of row r0 + RS i, piece ch of block db: two 16-byte chunks of the swizzled tile
+    auto store = [&](uint32_t tile, int i, int db, const uint32_t* x) {
+      const uint32_t b = tile + db * (kBN * 128) + i * (RS * 128);
+      sts128(b + sw_off(r0, 2 * ch), x[0], x[1], x[2], x[3]);
+      sts128(b + sw_off(r0, 2 * ch + 1), x[4], x[5], x[6], x[7]);
+    };
+    uint32_t ksc = 0, vsc = 0;
+    int vref = -1;
+    auto fetch_scales = [&](const uint8_t* scales, int t) -> uint32_t {  // bytes of tokens 4 lane .. 4 lane + 3
+      const int page = lane * 4 < rt.kv_end - (tile0 + t) * kBN ? page_at(t * (kBN / kPage) + lane / 4) : -1;
+      return page < 0 ? 0u : __ldg(reinterpret_cast<const uint32_t*>(scales + page * p.scale_stride + hkv * kPage) + lane % 4);
+    };
+    if (n_tiles > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        fetch(kp, 0, i);
+        cp_async_commit();
+      }
+      ksc = fetch_scales(p.ks, 0);
+      vsc = fetch_scales(p.vs, 0);
+    }
+    bool ok = true;
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      const int left = rt.kv_end - (tile0 + t) * kBN;
+      // ---- K ----
+      if (t >= kRing) ok = tc::mbar_wait(k_free(t), (t / kRing - 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      {
+        // the tile's largest key exponent, over live and finite rows
+        int emax = 0, vmax = 0;
+        uint32_t miss = 0, vnan = 0;
+        const bool there = lane * 4 < left && page_at(t * (kBN / kPage) + lane / 4) >= 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int kb = ksc >> (8 * i) & 0xff, vb = vsc >> (8 * i) & 0xff;
+          const bool live = there && lane * 4 + i < left;
+          if (live && kb != q8::kNanByte) emax = max(emax, kb);
+          if (lane * 4 + i < left && !there) miss |= 1u << i;
+          if (live && vb == q8::kNanByte) vnan |= 1u << i;
+          if (live && vb != q8::kNanByte) vmax = max(vmax, vb);
+        }
+        emax = __reduce_max_sync(0xffffffffu, emax);
+        vmax = __reduce_max_sync(0xffffffffu, vmax);
+        // all four warps come to the same reference: it moves when the largest scale leaves fp16's range above it
+        if (vref < 0 || vmax > vref + kVHead) vref = max(vmax - kVHead, 0);
+        const bool special = __any_sync(0xffffffffu, (miss | vnan) != 0);
+        TileInfo& info = s_info[t % kInfo];
+        if (ct == 0) {
+          info.scale = p.scale_log2 * q8::scale_of(emax);
+          info.vref = vref;
+          info.special = special;
+        }
+        if (special && warp == kConvWarp) {  // bits of tokens 4 lane .. + 3 into words of 32
+          miss <<= (lane & 7) * 4, vnan <<= (lane & 7) * 4;
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) {
+            miss |= __shfl_xor_sync(0xffffffffu, miss, o);
+            vnan |= __shfl_xor_sync(0xffffffffu, vnan, o);
+          }
+          if ((lane & 7) == 0) info.missing[lane >> 3] = miss, info.vnan[lane >> 3] = vnan;
+        }
+        const uint32_t dst = ks + (t % kRing) * L::kKV;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int kb = byte_of_row(ksc, i);
+          const uint32_t f = f16_pow2(min(kb - emax, 0));
+          cp_async_wait<N - 1>();  // the oldest of the N rows on their way
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const uint4 c = lds128(stage + (i * DB + db) * kSlot);
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+            uint32_t x[8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              q8::e4m3x4_to_f16x4(w[u], x[2 * u], x[2 * u + 1]);  // NaN codes stay NaN
+              x[2 * u] = hmul2(x[2 * u], f);
+              x[2 * u + 1] = hmul2(x[2 * u + 1], f);
+            }
+            store(dst, i, db, x);
+          }
+          fetch(vp, t, i);
+          cp_async_commit();
+        }
+      }
+      tc::fence_proxy_async_smem();
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(k_full(t)) : "memory");
+      if (t + 1 < n_tiles) ksc = fetch_scales(p.ks, t + 1);
+      // ---- V ----
+      if (t >= kRing) ok = tc::mbar_wait(v_free(t), (t / kRing - 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      {
+        const uint32_t dst = vs + (t % kRing) * L::kKV;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int vb = byte_of_row(vsc, i);
+          // a NaN row (and what a dead row's byte may say) counts as zeros: its codes are taken out
+          const uint32_t f = f16_pow2(min(vb - vref, kVHead));
+          const uint32_t keep = vb == q8::kNanByte ? 0u : 0xffffffffu;
+          cp_async_wait<N - 1>();
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const uint4 c = lds128(stage + (i * DB + db) * kSlot);
+            const uint32_t w[4] = {c.x & keep, c.y & keep, c.z & keep, c.w & keep};
+            uint32_t x[8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              q8::e4m3x4_to_f16x4(w[u], x[2 * u], x[2 * u + 1]);
+              x[2 * u] = hmul2(x[2 * u], f);
+              x[2 * u + 1] = hmul2(x[2 * u + 1], f);
+            }
+            store(dst, i, db, x);
+          }
+          if (t + 1 < n_tiles) fetch(kp, t + 1, i);
+          cp_async_commit();
+        }
+      }
+      tc::fence_proxy_async_smem();
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(v_full(t)) : "memory");
+      if (t + 1 < n_tiles) vsc = fetch_scales(p.vs, t + 1);
+    }
+    cp_async_wait<0>();
+  } else if (warp >= kMmaWarp) {
+    // =================== MMA issue (the first warp of its group; the others wait at the end) ===================
+    regs_dec<kRegsMma>();
+    const uint32_t id_s = tc::idesc_f16(false, false, false, kBM, kBN);
+    const uint32_t id_o = tc::idesc_f16(false, false, true, kBM, D);
+    const uint64_t dq0 = tc::smem_desc_sw128(qs, 16, 1024);
+    const uint64_t dk0 = tc::smem_desc_sw128(ks, 16, 1024);
+    const uint64_t dv0 = tc::smem_desc_sw128(vs, kBN * 128, 1024);
+    auto issue_s = [&](int g, int t) {
+      tc::tc_fence_after();
+      const uint64_t qb = dq0 + (p.alt ? 0u : static_cast<uint64_t>((g * L::kQ) >> 4));
+      const uint64_t kb = dk0 + static_cast<uint64_t>(((t % kRing) * L::kKV) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * (kBM * 128) + (kk & 3) * 32) >> 4);
+        tc::mma_f16(t_s(g), qb + off, kb + off, id_s, kk > 0 ? 1u : 0u);
+      }
+      tc::mma_commit(s_full(g));
+      if (p.alt || g == 1) tc::mma_commit(k_free(t));
+    };
+    auto issue_o = [&](int g, int k, int t) {
+      tc::tc_fence_after();
+      const uint64_t vb = dv0 + static_cast<uint64_t>(((t % kRing) * L::kKV) >> 4);
+#pragma unroll
+      for (int part = 0; part < (kTwoParts ? 2 : 1); ++part) {
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk) {
+          const uint32_t pa = t_s(g) + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8;
+          tc::mma_f16_ts(t_o(g), pa, vb + static_cast<uint64_t>((kk * 16 * 128) >> 4), id_o,
+                         (k > 0 || part > 0 || kk > 0) ? 1u : 0u);
+        }
+      }
+      tc::mma_commit(o_done(g));
+      if (p.alt || g == 1) tc::mma_commit(v_free(t));
+    };
+    bool ok = warp == kMmaWarp;
+    for (int g = 0; ok && g < 2; ++g) {
+      const int t = tile_at(g, 0);
+      if (t >= n_tiles) break;
+      ok = tc::mbar_wait(k_full(t), (t / kRing) & 1);
+      if (ok && lane == 0) issue_s(g, t);
+      __syncwarp();
+    }
+    for (int k = 0; ok && tile_at(0, k) < n_tiles; ++k) {
+      for (int g = 0; ok && g < 2; ++g) {
+        const int t = tile_at(g, k), tn = tile_at(g, k + 1);
+        if (t >= n_tiles) break;
+        ok = tc::mbar_wait(p_full(g), k & 1) && tc::mbar_wait(v_full(t), (t / kRing) & 1);
+        if (!ok) break;
+        if (lane == 0) issue_o(g, k, t);
+        __syncwarp();
+        if (tn < n_tiles) {  // S_g overwrites P_g: once PV_g has read it
+          ok = tc::mbar_wait(k_full(tn), (tn / kRing) & 1) && tc::mbar_wait(o_done(g), k & 1);
+          if (!ok) break;
+          if (lane == 0) issue_s(g, tn);
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // =================== softmax ===================
+    regs_inc<kRegsSoftmax>();
+    const int g = warp / kGroupWarps;
+    const int half = (warp % kGroupWarps) / 4, rq = warp % 4;
+    const int row = rq * 32 + lane;  // of the group, and TMEM lane
+    const int r = rt.row0 + (p.alt ? 0 : g * kBM) + row;
+    const bool valid = r < rt.n_rows;
+    const int tok = valid ? r / p.n_rep : 0;
+    const int len = __ldg(p.lens + rt.b);
+    // last visible token, from the split's first
+    const int lim = (valid ? min(p.causal ? len - rt.n_q + tok : len - 1, rt.kv_end - 1) : rt.kv_end - 1) - tile0 * kBN;
+    const uint32_t lane_base = static_cast<uint32_t>(rq * 32) << 16;
+    constexpr int kSC = kBN / 2, kOC = D / 2;
+    const int sc0 = half * kSC, oc0 = half * kOC;
+    const uint32_t ts = t_s(g) + lane_base + sc0, to = t_o(g) + lane_base + oc0;
+    const uint32_t bar_id = 2 + g * 4 + rq;  // the two warps that share these rows
+    float* mxg = s_mx + g * 4 * kBM;
+    const float qf = s_qf[(p.alt ? 0 : g * kBM) + row];
+    float m_ref = -INFINITY, l_run = 0.f;
+    int vref = -1;  // reference of the values in O
+    bool failed = false, row_nan = false;
+    // a wait that runs out only sets `failed`: every warp still reaches every barrier
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (failed) return;
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(bar, parity))) failed = true;
+    };
+    int k = 0;
+    for (; tile_at(g, k) < n_tiles; ++k) {
+      const int t = tile_at(g, k);
+      wait(s_full(g), k & 1);
+      tc::tc_fence_after();
+      const TileInfo& info = s_info[t % kInfo];
+      const float scale = info.scale * qf;
+      const int tbase = t * kBN + sc0;
+      const bool crosses = tbase + kSC - 1 > lim;
+      const bool special = info.special != 0;
+      auto mask32 = [&](float* s, int c0) {  // columns c0 .. c0 + 31 of this thread's half
+        if (crosses) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[c] = (tbase + c0 + c <= lim) ? s[c] : -INFINITY;
+        }
+        if (special) {
+          const uint32_t miss = info.missing[(sc0 + c0) >> 5];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[c] = (miss >> c & 1) ? -INFINITY : s[c];
+        }
+      };
+      // pass 1: row maximum; columns [32, 64) stay in registers for pass 2
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float s1[32];
+      {
+        float s0[32];
+        tc::tmem_ld32x2(ts, ts + 32, s0, s1);
+        mask32(s0, 0);
+        mask32(s1, 32);
+        if (special) {  // rows that see a NaN value row
+          const uint32_t n0 = info.vnan[sc0 >> 5], n1 = info.vnan[(sc0 + 32) >> 5];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            row_nan |= (n0 >> c & 1) && s0[c] != -INFINITY;
+            row_nan |= (n1 >> c & 1) && s1[c] != -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          mx4[c & 3] = fmaxf(mx4[c & 3], s0[c]);
+          mx4[c & 3] = fmaxf(mx4[c & 3], s1[c]);
+        }
+      }
+      const float mxh = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      mxg[((k & 1) * 2 + half) * kBM + row] = mxh;
+      asm volatile("bar.sync %0, %1;\n" ::"r"(bar_id), "n"(64) : "memory");
+      const float mx = fmaxf(mxg[((k & 1) * 2) * kBM + row], mxg[((k & 1) * 2 + 1) * kBM + row]) * scale;
+      const bool need = mx > m_ref + kRescale;
+      float alpha = 1.f;
+      bool rescale = false;
+      if (need) {
+        alpha = fast_exp2(m_ref - mx);
+        m_ref = mx;
+        l_run *= alpha;
+      }
+      if (info.vref != vref) {  // the same for the whole warp
+        if (k > 0) alpha *= exp2f(static_cast<float>(vref - info.vref));
+        rescale = k > 0;
+        vref = info.vref;
+      }
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref - kWOff;
+      const uint64_t sc2 = pk2(scale, scale), nm2 = pk2(-m_use, -m_use);
+      uint64_t sum2[2] = {0ull, 0ull};
+      // pass 2: S columns [c0, c0 + 32) -> weights, high then low parts, in the same TMEM columns
+      auto emit = [&](int c0, float* s) {
+        uint32_t hi[16];
+        [[maybe_unused]] uint32_t lo[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const uint64_t x2 = fma2(pk2(s[c], s[c + 1]), sc2, nm2);
+          uint64_t e2;
+          if ((c >> 1) % kEmuStride == kEmuStride - 1) {
+            e2 = exp2_poly2(x2);
+          } else {
+            float xa, xb;
+            up2(x2, xa, xb);
+            e2 = pk2(fast_exp2(xa), fast_exp2(xb));
+          }
+          sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], e2);
+          float ea, eb;
+          up2(e2, ea, eb);
+          if constexpr (kTwoParts) {
+            split2<__half>(ea, eb, hi[c >> 1], lo[c >> 1]);
+          } else {
+            hi[c >> 1] = pack2<__half>(ea, eb);
+          }
+        }
+        tc::tmem_st16_nowait(ts + c0, hi);
+        if constexpr (kTwoParts) tc::tmem_st16_nowait(ts + c0 + 16, lo);
+      };
+      emit(32, s1);
+      {
+        float s0[32];
+        tc::tmem_ld32(ts, s0);
+        mask32(s0, 0);
+        emit(0, s0);
+      }
+      if (rescale || (k > 0 && __any_sync(0xffffffffu, need))) {
+#pragma unroll
+        for (int c0 = 0; c0 < kOC; c0 += 32) {
+          float o[32];
+          tc::tmem_ld32(to + c0, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= alpha;
+          tc::tmem_st32u(to + c0, reinterpret_cast<const uint32_t*>(o));
+        }
+      }
+      tc::tmem_st_wait();
+      {
+        float sa, sb;
+        up2(add2(sum2[0], sum2[1]), sa, sb);
+        l_run += sa + sb;
+      }
+      tc::tc_fence_before();
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(p_full(g)) : "memory");
+    }
+    if (k > 0) wait(o_done(g), (k - 1) & 1);
+    // ---- epilogue ----
+    float* lg = s_l + g * 2 * kBM;
+    lg[half * kBM + row] = l_run;
+    mxg[((k & 1) * 2 + half) * kBM + row] = row_nan ? 1.f : 0.f;  // the buffer the last tile did not use
+    asm volatile("bar.sync %0, %1;\n" ::"r"(bar_id), "n"(64) : "memory");
+    const float l_row = lg[row] + lg[kBM + row];
+    const bool bad = mxg[((k & 1) * 2) * kBM + row] + mxg[((k & 1) * 2 + 1) * kBM + row] > 0.f;
+    const bool all_ok = __all_sync(0xffffffffu, !failed);
+    const bool none = l_row == 0.f;  // this part sees no token
+    const float nan = __int_as_float(0x7fc00000);
+    // l holds 2^kWOff times the sum; O the same times 2^-(vref - 127)
+    const float inv = none ? 0.f : (bad || !all_ok) ? nan : 1.f / l_row;
+    const float lse = !all_ok ? nan : none ? -INFINITY : (m_ref - kWOff + log2f(l_row)) * kLn2;
+    const int vexp = vref - 127;
+    const int64_t o = static_cast<int64_t>(rt.q0 + tok) * p.Hq + hkv * p.n_rep + (valid ? r % p.n_rep : 0);
+    const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
+    const int part = p.alt ? 2 * split + g : split;
+    if (all_ok && k > 0) tc::tc_fence_after();
+#pragma unroll
+    for (int c0 = 0; c0 < kOC; c0 += 32) {
+      float acc[32];
+      if (all_ok && k > 0) {
+        tc::tmem_ld32(to + c0, acc);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+      }
+      if (valid) {
+        if (p.parts == 1) {
+          T* dst = static_cast<T*>(p.out) + o * D + oc0 + c0;
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = none && all_ok ? 0.f : scalbnf(acc[c + i] * inv, vexp);
+            *reinterpret_cast<uint4*>(dst + c) =
+                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+          }
+        } else {
+          float* dst = p.part_o + (part * all_rows + o) * D + oc0 + c0;
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            *reinterpret_cast<float4*>(dst + c) = make_float4(scalbnf(acc[c] * inv, vexp), scalbnf(acc[c + 1] * inv, vexp),
+                                                              scalbnf(acc[c + 2] * inv, vexp), scalbnf(acc[c + 3] * inv, vexp));
+        }
+      }
+    }
+    if (valid && half == 0) {
+      if (p.parts > 1) p.part_lse[part * all_rows + o] = lse;
+      else if (p.lse_out != nullptr) p.lse_out[o] = lse;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the parts of every row; one warp per row, D / 32 columns a lane.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) chunk_q8_merge_kernel(const __grid_constant__ ChunkQ8Params p) {
+  constexpr int C = D / 32;
+  pdl_wait();
+  const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
+  const int64_t o = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (o >= all_rows || q8::request_of(p.cu_q, p.B, static_cast<int>(o / p.Hq)) < 0) return;
+  float M = -INFINITY;
+  bool nan = false;
+  for (int i = lane; i < p.parts; i += 32) {
+    const float x = p.part_lse[i * all_rows + o];
+    nan |= x != x;
+    M = fmaxf(M, x);
+  }
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  nan = __any_sync(0xffffffffu, nan);
+  float a[C] = {}, W = 0.f;
+  if (M != -INFINITY) {
+#pragma unroll 4
+    for (int i = 0; i < p.parts; ++i) {
+      const float x = p.part_lse[i * all_rows + o];
+      if (x == -INFINITY) continue;
+      const float w = exp2f((x - M) * 1.4426950408889634f);
+      W += w;
+      const float* src = p.part_o + (i * all_rows + o) * D + lane * C;
+#pragma unroll
+      for (int k = 0; k < C; ++k) a[k] += w * src[k];
+    }
+  }
+  const float inv = nan ? __int_as_float(0x7fc00000) : M == -INFINITY ? 0.f : 1.f / W;
+  T* dst = static_cast<T*>(p.out) + o * D + lane * C;
+#pragma unroll
+  for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(a[k] * inv, a[k + 1] * inv);
+  if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = nan ? inv : M == -INFINITY ? -INFINITY : M + logf(W);
+}
+
+template <typename T, int D>
+int launch(const ChunkQ8Params& p, cudaStream_t st) {
+  auto kern = chunk_q8_kernel<T, D>;
+  static bool raised[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !raised[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes) != cudaSuccess) {
+      set_error("q8_attention_launch:smem_attr");
+      return BPKV_ERR_CUDA;
+    }
+    if (dev >= 0 && dev < 64) raised[dev] = true;
+  }
+  kern<<<static_cast<unsigned>(p.B * p.tiles * p.splits * p.Hkv), kThreads, Layout<D>::kBytes, st>>>(p);
+  if (p.parts > 1) {
+    const int64_t rows = static_cast<int64_t>(p.total_q) * p.Hq;
+    const cudaError_t e = launch_pdl(chunk_q8_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, p);
+    if (e != cudaSuccess) {
+      set_error("q8_attention_launch:%s", cudaGetErrorString(e));
+      return BPKV_ERR_CUDA;
+    }
+  }
+  BPKV_RETURN_LAUNCH("q8_attention_launch");
+}
+
+}  // namespace
+
+int chunk_q8_tc_launch(const ChunkQ8Params& p, int head_dim, int dtype, cudaStream_t st) {
+  if (dtype == BPKV_BF16) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, st) : launch<__nv_bfloat16, 128>(p, st);
+  return head_dim == 64 ? launch<__half, 64>(p, st) : launch<__half, 128>(p, st);
+}
+
+}  // namespace bpkv

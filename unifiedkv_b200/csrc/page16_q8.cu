@@ -40,6 +40,7 @@
 
 #include <type_traits>
 
+#include "chunk_q8.cuh"
 #include "q8.cuh"
 
 namespace bpkv {
@@ -649,16 +650,38 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 constexpr int kMaxSplitItems = 4096;  // items whose page counts fit beside the ring in shared memory
 
+// Rows per request and KV head above which the tensor-core chunk kernel takes over.
+constexpr int kTcRows = 32;
+
 struct Plan {
+  int tc, alt, splits, parts;  // chunk_q8_tc.cu's, else the rest
   int nt, nw, ns, groups, hp, pl, grid, tiles, n_items, split;
   size_t lse_off, o_off, bytes;
 };
 
 // Rows per tile: the smallest of {8, 16, 512 * 8 / D} that holds a request's rows (a wider tile reads
 // K and V once for more rows; its accumulators are what the register file holds).
-Plan make_plan(int B, int Hkv, int n_rep, int D, int max_q) {
+Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max_blocks, float scale) {
   Plan pl{};
   const int64_t rows = static_cast<int64_t>(max_q) * n_rep;
+  if (D <= 128 && max_q > 1 && rows > kTcRows && scale > 0.f) {
+    pl.tc = 1;
+    pl.alt = rows <= 128;
+    const int64_t tiles = (rows + (pl.alt ? 127 : 255)) / (pl.alt ? 128 : 256);
+    const int64_t ctas = tiles * B * Hkv;
+    pl.tiles = static_cast<int>(tiles);
+    pl.n_items = tiles * B < (1LL << 30) && ctas < (1LL << 30) ? static_cast<int>(tiles * B) : -1;
+    // split the tokens where the row tiles alone leave SMs idle, down to 512 tokens a split
+    const int64_t fill = ctas > 0 ? sm_count() / ctas : 1, most = (static_cast<int64_t>(max_blocks) * kPage + 511) / 512;
+    pl.splits = static_cast<int>(max(static_cast<int64_t>(1), min(min(fill, most), static_cast<int64_t>(64))));
+    pl.parts = pl.splits * (pl.alt ? 2 : 1);
+    if (pl.parts > 1) {
+      const size_t all_rows = static_cast<size_t>(total_q) * Hkv * n_rep;
+      pl.o_off = up256(sizeof(float) * pl.parts * all_rows);
+      pl.bytes = pl.o_off + sizeof(float) * pl.parts * all_rows * D;
+    }
+    return pl;
+  }
   const int nt_max = 512 / D;
   pl.nt = rows <= 8 ? 1 : (rows <= 16 || nt_max == 2) ? 2 : nt_max;
   pl.nw = pl.nt == 1 ? 16 : 8;
@@ -737,31 +760,32 @@ int dispatch(Q8Params& p, const Plan& pl, int D, cudaStream_t st) {
 
 using namespace bpkv;
 
-extern "C" BPKV_API size_t bpkv_q8_attention_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim,
-                                                            int max_seqlen_q) {
-  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q <= 0 ||
+extern "C" BPKV_API size_t bpkv_q8_attention_workspace_size(int batch, int total_q, int num_q_heads, int num_kv_heads,
+                                                            int head_dim, int max_blocks, int max_seqlen_q,
+                                                            float softmax_scale) {
+  if (batch <= 0 || total_q <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q <= 0 ||
       !(head_dim == 64 || head_dim == 128 || head_dim == 256))
     return 0;
-  const Plan pl = make_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_seqlen_q);
-  return pl.bytes;
+  return make_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_seqlen_q, max_blocks, softmax_scale)
+      .bytes;
 }
 
 extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, const void* v_codes,
                                           const uint8_t* k_scales, const uint8_t* v_scales, const int32_t* block_table,
                                           const int32_t* cu_seqlens_q, const int32_t* seqlens_k, void* out,
-                                          float* lse_out, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                          float* lse_out, int batch, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
                                           int max_blocks, int num_pages, int max_seqlen_q, int64_t q_stride_t,
                                           int64_t q_stride_h, int64_t page_stride, int64_t scale_stride,
                                           int64_t bt_stride_b, float softmax_scale, int causal, int empty_nan,
                                           int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   const char* what = "q8_attention_shape_unsupported";
-  BPKV_CHECK_ARG(batch >= 0 && num_q_heads > 0 && max_blocks >= 0 && num_pages >= 0, "%s:empty", what);
+  BPKV_CHECK_ARG(batch >= 0 && total_q >= 0 && num_q_heads > 0 && max_blocks >= 0 && num_pages >= 0, "%s:empty", what);
   BPKV_CHECK_ARG(num_kv_heads > 0 && num_q_heads % num_kv_heads == 0, "%s:gqa", what);
   BPKV_CHECK_ARG(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s:head_dim_%d", what, head_dim);
   BPKV_CHECK_ARG(dtype == BPKV_F16 || dtype == BPKV_BF16, "%s:dtype_%d", what, dtype);
-  BPKV_CHECK_ARG(cu_seqlens_q != nullptr || max_seqlen_q == 1, "%s:max_seqlen_q", what);
-  if (batch == 0 || max_seqlen_q <= 0) return BPKV_OK;
+  BPKV_CHECK_ARG(cu_seqlens_q != nullptr || (max_seqlen_q == 1 && total_q == batch), "%s:max_seqlen_q", what);
+  if (batch == 0 || total_q == 0 || max_seqlen_q <= 0) return BPKV_OK;
   BPKV_CHECK_ARG(q && k_codes && v_codes && k_scales && v_scales && seqlens_k && out && (block_table || max_blocks == 0),
                  "%s:null_pointer", what);
   BPKV_CHECK_ARG(aligned16(q) && aligned16(k_codes) && aligned16(v_codes) && aligned16(k_scales) && aligned16(v_scales) &&
@@ -770,13 +794,47 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
                  "%s:alignment", what);
   BPKV_CHECK_ARG(max_blocks <= (1 << 26), "%s:max_blocks_%d", what, max_blocks);
   const int n_rep = num_q_heads / num_kv_heads;
-  const Plan pl = make_plan(batch, num_kv_heads, n_rep, head_dim, max_seqlen_q);
+  const Plan pl = make_plan(batch, total_q, num_kv_heads, n_rep, head_dim, max_seqlen_q, max_blocks, softmax_scale);
   BPKV_CHECK_ARG(pl.n_items > 0, "%s:max_seqlen_q", what);
   // the flattened page list is indexed in 31 bits
-  BPKV_CHECK_ARG(!pl.split || static_cast<int64_t>(pl.n_items) * max_blocks < (1LL << 31), "%s:max_blocks_%d", what, max_blocks);
+  BPKV_CHECK_ARG(pl.tc || !pl.split || static_cast<int64_t>(pl.n_items) * max_blocks < (1LL << 31), "%s:max_blocks_%d", what, max_blocks);
   if (pl.bytes > 0 && (workspace == nullptr || workspace_bytes < pl.bytes)) {
     set_error("q8_attention_workspace:need_%zu_bytes", pl.bytes);
     return BPKV_ERR_WORKSPACE;
+  }
+  if (pl.tc) {
+    ChunkQ8Params c{};
+    c.q = q;
+    c.kc = static_cast<const uint8_t*>(k_codes);
+    c.vc = static_cast<const uint8_t*>(v_codes);
+    c.ks = k_scales;
+    c.vs = v_scales;
+    c.bt = block_table;
+    c.cu_q = cu_seqlens_q;
+    c.lens = seqlens_k;
+    c.out = out;
+    c.lse_out = lse_out;
+    c.part_lse = static_cast<float*>(workspace);
+    c.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.o_off);
+    c.B = batch;
+    c.Hq = num_q_heads;
+    c.Hkv = num_kv_heads;
+    c.n_rep = n_rep;
+    c.tiles = pl.tiles;
+    c.splits = pl.splits;
+    c.parts = pl.parts;
+    c.alt = pl.alt;
+    c.causal = causal;
+    c.max_blocks = max_blocks;
+    c.num_pages = num_pages;
+    c.total_q = total_q;
+    c.q_st = q_stride_t;
+    c.q_sh = q_stride_h;
+    c.page_stride = page_stride;
+    c.scale_stride = scale_stride;
+    c.bt_sb = bt_stride_b;
+    c.scale_log2 = softmax_scale * 1.4426950408889634f;
+    return chunk_q8_tc_launch(c, head_dim, dtype, static_cast<cudaStream_t>(stream));
   }
   Q8Params p{};
   p.q = q;

@@ -21,6 +21,11 @@ where it lies below 2^-6 * 2^e.  A row with an infinity or a NaN is stored as Na
 
 A token costs 2 * kv_heads * (head_dim + 1) bytes.  head_dim is 64, 128 or 256.
 
+Attention computes on the stored values: scores, softmax and sums in fp32, the products on
+fp16 operands that hold the codes exactly.  A weight is rounded to 11 bits (22 for fp16
+results) and counts as zero below 2^-36 of the largest of its row, so a value 2^25 and
+more times larger than its neighbours can be lost where the row hardly looks at it.
+
 A page id outside the pool (-1 as of an offloaded page, or past its end) is never
 touched: tokens on such a page are not written, read back as zeros, and are left out of
 attention.  Every call runs on the current stream of its tensors' device without
@@ -225,12 +230,12 @@ def _attention(what: str, q: torch.Tensor, kv: QuantPagedKV, block_table: torch.
             return _attention(what, q, kv, bt, lens, cu, max_q, softmax_scale, n_rep, causal, lse_out)
     q = _aligned(q)
     out = torch.empty((total, h_q, d), dtype=q.dtype, device=dev)
-    ws_bytes = lib.bpkv_q8_attention_workspace_size(B, h_q, h_kv, d, max_q)
+    ws_bytes = lib.bpkv_q8_attention_workspace_size(B, total, h_q, h_kv, d, bt.shape[1], max_q, softmax_scale)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     qs = q.stride()
     rc = lib.bpkv_q8_attention(
         q.data_ptr(), kv.k_codes.data_ptr(), kv.v_codes.data_ptr(), kv.k_scales.data_ptr(), kv.v_scales.data_ptr(),
-        bt.data_ptr(), _lib.ptr(cu), lens.data_ptr(), out.data_ptr(), _lib.ptr(lse_out), B, h_q, h_kv, d, bt.shape[1],
+        bt.data_ptr(), _lib.ptr(cu), lens.data_ptr(), out.data_ptr(), _lib.ptr(lse_out), B, total, h_q, h_kv, d, bt.shape[1],
         n, max_q, qs[0], qs[1], kv.k_codes.stride(0), kv.k_scales.stride(0), bt.stride(0), float(softmax_scale),
         int(causal), int(cu is None), code, _lib.ptr(ws), ws_bytes, torch.cuda.current_stream(dev).cuda_stream)
     if rc:
