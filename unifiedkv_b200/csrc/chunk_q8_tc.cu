@@ -7,7 +7,7 @@
 // Design:
 //  * Bound.  A chunk does 4 * head_dim FLOP per (row, visible token): with hundreds of
 //    rows the tensor pipe and the exponentials bound it, not the pages' bytes.
-//  * Codes become fp16 operands on the way into shared memory.  Four converter warps
+//  * Codes become fp16 operands on the way into shared memory.  Eight converter warps
 //    bring 16-code pieces in by cp.async (one tile ahead, each thread its own), turn them
 //    into fp16 (cvt.rn.f16x2.e4m3x2 and one multiply per pair; e4m3 to bf16 takes five
 //    instructions a pair and made the converters the bound) and store them in the
@@ -45,22 +45,23 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kBM = 128, kBN = 128;   // rows of a group, tokens of a K/V tile
 constexpr int kRing = 2;              // K (and V) tiles in shared memory
 constexpr int kGroupWarps = 8;        // softmax warps of a group: warps 0 .. 15
-constexpr int kConvWarp = 16, kConvWarps = 4, kMmaWarp = 20;
-// Six warpgroups are launched with 80 registers a thread (61,440 in all) and share them out anew:
-// softmax 4 x 128 x 96, converters 128 x 64, MMA (and three idle warps) 128 x 32 = 61,440.
-constexpr int kThreads = 24 * 32;
-constexpr int kRegsSoftmax = 96, kRegsConv = 64, kRegsMma = 32;
-static_assert(128 * (4 * kRegsSoftmax + kRegsConv + kRegsMma) <= kThreads * 80, "register split");
-constexpr int kMaxPages = 2048;       // block-table entries staged in shared memory
+constexpr int kConvWarp = 16, kConvWarps = 8, kMmaWarp = 24, kScaleWarp = 25;
+// Seven warpgroups are launched with 72 registers a thread (64,512 in all) and share them out anew:
+// softmax 4 x 128 x 88, converters 2 x 128 x 56, MMA, scales (and two idle warps) 128 x 40 = 64,512.
+constexpr int kThreads = 28 * 32;
+constexpr int kRegsSoftmax = 88, kRegsConv = 56, kRegsMma = 40;
+static_assert(128 * (4 * kRegsSoftmax + 2 * kRegsConv + kRegsMma) <= kThreads * 72, "register split");
+constexpr int kMaxPages = 1024;       // block-table entries staged in shared memory
 constexpr int kMaxRanked = 512;       // row tiles ordered longest first
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescale = 4.f, kWOff = 11.f;  // weights <= 2^4, held times 2^11
 constexpr int kVHead = 6;                      // values are held as code * 2^(byte - vref), byte <= vref + 6
 constexpr int kEmuStride = 8;
 
-// What the softmax warps need to know of a K/V tile, in a ring of 4: a slot is written with K(t + 4),
-// which needs S(t + 2) issued, which needs the softmax of tile t + 1 done.
-struct TileInfo {
+// What a K/V tile's scales come to, worked out once by the scale warp: for the converters a factor per row
+// (fp16 bits), for the softmax warps the rest.  A ring of 4; a slot is free again once P.V of its tile is done.
+struct __align__(16) TileInfo {
+  uint16_t kf[kBN], vf[kBN];
   float scale;       // softmax scale * log2(e) * 2^(largest key exponent)
   int vref;          // reference byte of the values
   uint32_t special;  // a token is missing (no page) or its value row is NaN
@@ -69,18 +70,22 @@ struct TileInfo {
 };
 constexpr int kInfo = 4;
 
-template <int D>
+template <int D, bool ALT>
 struct Layout {
   static constexpr int kDB = D / 64;
+  static constexpr int kQTiles = ALT ? 1 : 2;  // alternating groups share their rows
+  // halves (the codes of one K or V tile) on their way to the converters: as many as fit.  Where few rows
+  // read a long cache (alternating), memory's latency is what they have to cover.
+  static constexpr int kDepth = D == 64 ? 6 : ALT ? 3 : 1;
   static constexpr int kQ = kDB * kBM * 128;   // bytes of a Q tile
   static constexpr int kKV = kDB * kBN * 128;  // bytes of a K or V tile
-  static constexpr int kBars = 2 * kQ + 2 * kRing * kKV;
+  static constexpr int kBars = kQTiles * kQ + 2 * kRing * kKV;
   static constexpr int kInfoOff = kBars + 256;
   static constexpr int kMx = kInfoOff + ((kInfo * static_cast<int>(sizeof(TileInfo)) + 15) / 16) * 16;
   static constexpr int kL = kMx + 4 * 2 * 2 * 2 * kBM;  // after the row maxima, [group][2 buffers][half][row]
   static constexpr int kQf = kL + 4 * 2 * 2 * kBM;      // after the row sums, [group][half][row]
   static constexpr int kStage = kQf + 4 * 2 * kBM;      // after q's row factors, [group][row]
-  static constexpr int kPages = kStage + kBN * D;       // after the codes of one tile, on their way to a converter
+  static constexpr int kPages = kStage + kDepth * kBN * D;
   static constexpr int kBytes = kPages + 4 * kMaxPages + 1024;  // + alignment
 };
 
@@ -114,12 +119,28 @@ __device__ __forceinline__ uint32_t f16_pow2(int e) {
   return x | x << 16;
 }
 
+// The MMAs with their descriptors as two 32-bit words: only the low one (address, leading offset) varies, and
+// an issuing thread with few registers keeps ahead of the tensor pipe.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate));
+}
+
 struct RowTile {
   int b, q0, n_q, n_rows, row0, kv_end;
 };
+template <bool ALT>
 __device__ __forceinline__ RowTile row_tile(const ChunkQ8Params& p, int i) {
   RowTile r;
-  const int rows = p.alt ? kBM : 2 * kBM;
+  const int rows = ALT ? kBM : 2 * kBM;
   r.b = i / p.tiles;
   r.row0 = (i % p.tiles) * rows;
   r.q0 = __ldg(p.cu_q + r.b);
@@ -134,14 +155,15 @@ __device__ __forceinline__ RowTile row_tile(const ChunkQ8Params& p, int i) {
   return r;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool ALT>
 __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_constant__ ChunkQ8Params p) {
-  using L = Layout<D>;
+  using L = Layout<D, ALT>;
+  static_assert(L::kBytes <= 232448, "shared memory");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t qs = smem_u32(smem), ks = qs + 2 * L::kQ, vs = ks + kRing * L::kKV;
+  const uint32_t qs = smem_u32(smem), ks = qs + L::kQTiles * L::kQ, vs = ks + kRing * L::kKV;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  constexpr int kBarCount = 4 * kRing + 6;
+  constexpr int kBarCount = 4 * kRing + 6 + 2 * kInfo;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBarCount);
   static_assert((kBarCount + 1) * 8 <= 256, "barrier area");
   TileInfo* s_info = reinterpret_cast<TileInfo*>(smem + L::kInfoOff);
@@ -159,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   int item = static_cast<int>(blockIdx.x / p.Hkv) / p.splits;
   if (n_items <= kMaxRanked) {
     __shared__ int s_item;
-    for (int i = tid; i < n_items; i += kThreads) s_pages[i] = row_tile(p, i).kv_end;
+    for (int i = tid; i < n_items; i += kThreads) s_pages[i] = row_tile<ALT>(p, i).kv_end;
     __syncthreads();
     for (int i = tid; i < n_items; i += kThreads) {
       const int wi = s_pages[i];
@@ -171,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     item = s_item;
     __syncthreads();  // s_pages is about to be filled
   }
-  const RowTile rt = row_tile(p, item);
+  const RowTile rt = row_tile<ALT>(p, item);
   if (rt.row0 >= rt.n_rows) return;  // uniform across the CTA, before any barrier or TMEM use
   const int all_tiles = (rt.kv_end + kBN - 1) / kBN;
   const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
@@ -185,6 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   auto s_full = [&](int g) { return smem_u32(&bars[4 * kRing + g]); };
   auto p_full = [&](int g) { return smem_u32(&bars[4 * kRing + 2 + g]); };
   auto o_done = [&](int g) { return smem_u32(&bars[4 * kRing + 4 + g]); };
+  auto info_full = [&](int t) { return smem_u32(&bars[4 * kRing + 6 + t % kInfo]); };
+  auto info_free = [&](int t) { return smem_u32(&bars[4 * kRing + 6 + kInfo + t % kInfo]); };
 
   if (warp == 0) {
     tc::tmem_alloc(smem_u32(tmem_slot), kTmemCols);
@@ -196,6 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       tc::mbar_init(v_full(i), 32u * kConvWarps);
       tc::mbar_init(k_free(i), 1u);
       tc::mbar_init(v_free(i), 1u);
+    }
+    for (int i = 0; i < kInfo; ++i) {
+      tc::mbar_init(info_full(i), 32u);
+      tc::mbar_init(info_free(i), 1u);
     }
     for (int g = 0; g < 2; ++g) {
       tc::mbar_init(s_full(g), 1u);
@@ -212,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   // ---- Q tiles -> shared memory as fp16, swizzled K-major; D / 8 neighbouring lanes share a row ----
   {
     constexpr int CPR = D / 8;
-    const int rows = p.alt ? kBM : 2 * kBM;
+    const int rows = ALT ? kBM : 2 * kBM;
     for (int e = tid; e < rows * CPR; e += kThreads) {  // kThreads and rows * CPR are multiples of 32
       const int m = e / CPR, ch = e % CPR, r = rt.row0 + m;
       uint4 raw = make_uint4(0, 0, 0, 0);
@@ -244,8 +272,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   const uint32_t tmem = *tmem_slot;
   auto t_s = [&](int g) { return tmem + static_cast<uint32_t>(g * 256); };
   auto t_o = [&](int g) { return tmem + static_cast<uint32_t>(g * 256 + 128); };
+  const bool staged = n_tiles * (kBN / kPage) <= kMaxPages;
+  auto page_at = [&](int idx) {  // idx from page0
+    return staged || idx < kMaxPages ? s_pages[idx] : q8::page_of(bt_row, page0 + idx, p.max_blocks, p.num_pages);
+  };
   // group g's tile number k is K/V tile tile_at(g, k)
-  auto tile_at = [&](int g, int k) { return p.alt ? 2 * k + g : k; };
+  auto tile_at = [&](int g, int k) { return ALT ? 2 * k + g : k; };
 
   if (warp >= kConvWarp && warp < kMmaWarp) {
     // =================== converters ===================
@@ -258,21 +290,22 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     const int ch = ct & 3, r0 = ct >> 2;
     const int64_t in_page = static_cast<int64_t>(r0 & 15) * p.Hkv * D + static_cast<int64_t>(hkv) * D + ch * 16;
     const uint8_t *kp = p.kc + in_page, *vp = p.vc + in_page;
-    const bool staged = n_tiles * (kBN / kPage) <= kMaxPages;
-    auto page_at = [&](int idx) {  // idx from page0
-      return staged || idx < kMaxPages ? s_pages[idx] : q8::page_of(bt_row, page0 + idx, p.max_blocks, p.num_pages);
-    };
+    // Half 2t is K of tile t, half 2t + 1 its V; half h lies in slot h % kDepth of the staging area, where
+    // each thread keeps its own pieces.  Row i of half h + kDepth is fetched when that of half h is stored.
+    constexpr int kDepth = L::kDepth;
     const uint32_t stage = smem_u32(smem + L::kStage) + ct * 16;
-    // this thread's pieces of row r0 + RS i of a tile into its slots i of the staging area
-    auto fetch = [&](const uint8_t* base, int t, int i) {
-      const int page = page_at(t * (kBN / kPage) + RS / 16 * i + (r0 >> 4));
-      const bool ok = r0 + RS * i < rt.kv_end - (tile0 + t) * kBN && page >= 0;
-      const uint8_t* src = base + (ok ? page * p.page_stride : 0);
+    const int n_halves = 2 * n_tiles;
+    auto slot_of = [&](int h, int i) { return stage + ((h % kDepth * N + i) * DB) * kSlot; };
+    auto fetch = [&](int h, int i) {
+      if (h < n_halves) {
+        const int t = h >> 1;
+        const int page = page_at(t * (kBN / kPage) + RS / 16 * i + (r0 >> 4));
+        const bool ok = r0 + RS * i < rt.kv_end - (tile0 + t) * kBN && page >= 0;
+        const uint8_t* src = (h & 1 ? vp : kp) + (ok ? page * p.page_stride : 0);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) cp_async16(stage + (i * DB + db) * kSlot, src + db * 64, ok);
-    };
-    auto byte_of_row = [&](uint32_t sc, int i) {
-      return static_cast<int>(__shfl_sync(0xffffffffu, sc, (r0 >> 2) + RS / 4 * i) >> ((r0 & 3) * 8) & 0xffu);
+        for (int db = 0; db < DB; ++db) cp_async16(slot_of(h, i) + db * kSlot, src + db * 64, ok);
+      }
+      cp_async_commit();
     };
     // 16 values of row r0 + RS i, piece ch of block db: two 16-byte chunks of the swizzled tile
     auto store = [&](uint32_t tile, int i, int db, const uint32_t* x) {
@@ -280,70 +313,30 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       sts128(b + sw_off(r0, 2 * ch), x[0], x[1], x[2], x[3]);
       sts128(b + sw_off(r0, 2 * ch + 1), x[4], x[5], x[6], x[7]);
     };
-    uint32_t ksc = 0, vsc = 0;
-    int vref = -1;
-    auto fetch_scales = [&](const uint8_t* scales, int t) -> uint32_t {  // bytes of tokens 4 lane .. 4 lane + 3
-      const int page = lane * 4 < rt.kv_end - (tile0 + t) * kBN ? page_at(t * (kBN / kPage) + lane / 4) : -1;
-      return page < 0 ? 0u : __ldg(reinterpret_cast<const uint32_t*>(scales + page * p.scale_stride + hkv * kPage) + lane % 4);
-    };
-    if (n_tiles > 0) {
+    for (int h = 0; h < kDepth; ++h) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        fetch(kp, 0, i);
-        cp_async_commit();
-      }
-      ksc = fetch_scales(p.ks, 0);
-      vsc = fetch_scales(p.vs, 0);
+      for (int i = 0; i < N; ++i) fetch(h, i);
     }
     bool ok = true;
     for (int t = 0; ok && t < n_tiles; ++t) {
-      const int left = rt.kv_end - (tile0 + t) * kBN;
+      const TileInfo& info = s_info[t % kInfo];
+      auto factor = [&](const uint16_t* f, int i) {
+        const uint32_t x = f[r0 + RS * i];
+        return x | x << 16;
+      };
+      ok = tc::mbar_wait(info_full(t), (t / kInfo) & 1);
       // ---- K ----
-      if (t >= kRing) ok = tc::mbar_wait(k_free(t), (t / kRing - 1) & 1);
+      if (ok && t >= kRing) ok = tc::mbar_wait(k_free(t), (t / kRing - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
       {
-        // the tile's largest key exponent, over live and finite rows
-        int emax = 0, vmax = 0;
-        uint32_t miss = 0, vnan = 0;
-        const bool there = lane * 4 < left && page_at(t * (kBN / kPage) + lane / 4) >= 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kb = ksc >> (8 * i) & 0xff, vb = vsc >> (8 * i) & 0xff;
-          const bool live = there && lane * 4 + i < left;
-          if (live && kb != q8::kNanByte) emax = max(emax, kb);
-          if (lane * 4 + i < left && !there) miss |= 1u << i;
-          if (live && vb == q8::kNanByte) vnan |= 1u << i;
-          if (live && vb != q8::kNanByte) vmax = max(vmax, vb);
-        }
-        emax = __reduce_max_sync(0xffffffffu, emax);
-        vmax = __reduce_max_sync(0xffffffffu, vmax);
-        // all four warps come to the same reference: it moves when the largest scale leaves fp16's range above it
-        if (vref < 0 || vmax > vref + kVHead) vref = max(vmax - kVHead, 0);
-        const bool special = __any_sync(0xffffffffu, (miss | vnan) != 0);
-        TileInfo& info = s_info[t % kInfo];
-        if (ct == 0) {
-          info.scale = p.scale_log2 * q8::scale_of(emax);
-          info.vref = vref;
-          info.special = special;
-        }
-        if (special && warp == kConvWarp) {  // bits of tokens 4 lane .. + 3 into words of 32
-          miss <<= (lane & 7) * 4, vnan <<= (lane & 7) * 4;
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) {
-            miss |= __shfl_xor_sync(0xffffffffu, miss, o);
-            vnan |= __shfl_xor_sync(0xffffffffu, vnan, o);
-          }
-          if ((lane & 7) == 0) info.missing[lane >> 3] = miss, info.vnan[lane >> 3] = vnan;
-        }
         const uint32_t dst = ks + (t % kRing) * L::kKV;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int kb = byte_of_row(ksc, i);
-          const uint32_t f = f16_pow2(min(kb - emax, 0));
-          cp_async_wait<N - 1>();  // the oldest of the N rows on their way
+          const uint32_t f = factor(info.kf, i);
+          cp_async_wait<kDepth * N - 1>();  // the oldest row on its way has come
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            const uint4 c = lds128(stage + (i * DB + db) * kSlot);
+            const uint4 c = lds128(slot_of(2 * t, i) + db * kSlot);
             const uint32_t w[4] = {c.x, c.y, c.z, c.w};
             uint32_t x[8];
 #pragma unroll
@@ -354,13 +347,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
             }
             store(dst, i, db, x);
           }
-          fetch(vp, t, i);
-          cp_async_commit();
+          fetch(2 * t + kDepth, i);
         }
       }
       tc::fence_proxy_async_smem();
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(k_full(t)) : "memory");
-      if (t + 1 < n_tiles) ksc = fetch_scales(p.ks, t + 1);
       // ---- V ----
       if (t >= kRing) ok = tc::mbar_wait(v_free(t), (t / kRing - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -368,14 +359,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
         const uint32_t dst = vs + (t % kRing) * L::kKV;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int vb = byte_of_row(vsc, i);
-          // a NaN row (and what a dead row's byte may say) counts as zeros: its codes are taken out
-          const uint32_t f = f16_pow2(min(vb - vref, kVHead));
-          const uint32_t keep = vb == q8::kNanByte ? 0u : 0xffffffffu;
-          cp_async_wait<N - 1>();
+          uint32_t f = factor(info.vf, i);
+          const uint32_t keep = f == 0x7fff7fffu ? 0u : 0xffffffffu;  // a NaN row: its codes are taken out
+          f &= keep;
+          cp_async_wait<kDepth * N - 1>();
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
-            const uint4 c = lds128(stage + (i * DB + db) * kSlot);
+            const uint4 c = lds128(slot_of(2 * t + 1, i) + db * kSlot);
             const uint32_t w[4] = {c.x & keep, c.y & keep, c.z & keep, c.w & keep};
             uint32_t x[8];
 #pragma unroll
@@ -386,50 +376,109 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
             }
             store(dst, i, db, x);
           }
-          if (t + 1 < n_tiles) fetch(kp, t + 1, i);
-          cp_async_commit();
+          fetch(2 * t + 1 + kDepth, i);
         }
       }
       tc::fence_proxy_async_smem();
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(v_full(t)) : "memory");
-      if (t + 1 < n_tiles) vsc = fetch_scales(p.vs, t + 1);
     }
     cp_async_wait<0>();
   } else if (warp >= kMmaWarp) {
-    // =================== MMA issue (the first warp of its group; the others wait at the end) ===================
+    // =================== MMA issue, scales (the first two warps of the group) ===================
     regs_dec<kRegsMma>();
     const uint32_t id_s = tc::idesc_f16(false, false, false, kBM, kBN);
     const uint32_t id_o = tc::idesc_f16(false, false, true, kBM, D);
-    const uint64_t dq0 = tc::smem_desc_sw128(qs, 16, 1024);
-    const uint64_t dk0 = tc::smem_desc_sw128(ks, 16, 1024);
-    const uint64_t dv0 = tc::smem_desc_sw128(vs, kBN * 128, 1024);
+    const uint64_t dv = tc::smem_desc_sw128(vs, kBN * 128, 1024);  // the high words are all alike
+    const uint32_t hi = static_cast<uint32_t>(dv >> 32), v_lo = static_cast<uint32_t>(dv);
+    const uint32_t q_lo = static_cast<uint32_t>(tc::smem_desc_sw128(qs, 16, 1024));
+    constexpr uint32_t kToK = (L::kQTiles * L::kQ) >> 4;  // from Q's descriptor to K's
     auto issue_s = [&](int g, int t) {
       tc::tc_fence_after();
-      const uint64_t qb = dq0 + (p.alt ? 0u : static_cast<uint64_t>((g * L::kQ) >> 4));
-      const uint64_t kb = dk0 + static_cast<uint64_t>(((t % kRing) * L::kKV) >> 4);
+      const uint32_t qb = q_lo + (ALT ? 0u : static_cast<uint32_t>(g * (L::kQ >> 4)));
+      const uint32_t kb = q_lo + kToK + static_cast<uint32_t>((t % kRing) * (L::kKV >> 4));
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * (kBM * 128) + (kk & 3) * 32) >> 4);
-        tc::mma_f16(t_s(g), qb + off, kb + off, id_s, kk > 0 ? 1u : 0u);
+        const uint32_t off = static_cast<uint32_t>(((kk >> 2) * (kBM * 128) + (kk & 3) * 32) >> 4);
+        mma_ss(t_s(g), qb + off, kb + off, hi, id_s, kk > 0 ? 1u : 0u);
       }
       tc::mma_commit(s_full(g));
-      if (p.alt || g == 1) tc::mma_commit(k_free(t));
+      if (ALT || g == 1) tc::mma_commit(k_free(t));
     };
     auto issue_o = [&](int g, int k, int t) {
       tc::tc_fence_after();
-      const uint64_t vb = dv0 + static_cast<uint64_t>(((t % kRing) * L::kKV) >> 4);
+      const uint32_t vb = v_lo + static_cast<uint32_t>((t % kRing) * (L::kKV >> 4));
 #pragma unroll
       for (int part = 0; part < (kTwoParts ? 2 : 1); ++part) {
 #pragma unroll
         for (int kk = 0; kk < kBN / 16; ++kk) {
           const uint32_t pa = t_s(g) + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8;
-          tc::mma_f16_ts(t_o(g), pa, vb + static_cast<uint64_t>((kk * 16 * 128) >> 4), id_o,
-                         (k > 0 || part > 0 || kk > 0) ? 1u : 0u);
+          mma_ts(t_o(g), pa, vb + static_cast<uint32_t>((kk * 16 * 128) >> 4), hi, id_o, (k > 0 || part > 0 || kk > 0) ? 1u : 0u);
         }
       }
       tc::mma_commit(o_done(g));
-      if (p.alt || g == 1) tc::mma_commit(v_free(t));
+      if (ALT || g == 1) {
+        tc::mma_commit(v_free(t));
+        tc::mma_commit(info_free(t));
+      }
     };
+    if (warp == kScaleWarp) {
+      auto fetch_scales = [&](const uint8_t* scales, int t) -> uint32_t {  // bytes of tokens 4 lane .. 4 lane + 3
+        const int page = lane * 4 < rt.kv_end - (tile0 + t) * kBN ? page_at(t * (kBN / kPage) + lane / 4) : -1;
+        return page < 0 ? 0u : __ldg(reinterpret_cast<const uint32_t*>(scales + page * p.scale_stride + hkv * kPage) + lane % 4);
+      };
+      int vref = -1;
+      uint32_t ksc = 0, vsc = 0, ksc_next = 0, vsc_next = 0;  // of tiles t, t + 1
+      if (n_tiles > 0) ksc = fetch_scales(p.ks, 0), vsc = fetch_scales(p.vs, 0);
+      if (n_tiles > 1) ksc_next = fetch_scales(p.ks, 1), vsc_next = fetch_scales(p.vs, 1);
+      for (int t = 0; t < n_tiles; ++t) {
+        if (t >= kInfo && !__all_sync(0xffffffffu, tc::mbar_wait(info_free(t), (t / kInfo - 1) & 1))) break;
+        const int left = rt.kv_end - (tile0 + t) * kBN;
+        const bool there = lane * 4 < left && page_at(t * (kBN / kPage) + lane / 4) >= 0;
+        int emax = 0, vmax = 0;  // over live and finite rows
+        uint32_t miss = 0, vnan = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int kb = ksc >> (8 * i) & 0xff, vb = vsc >> (8 * i) & 0xff;
+          const bool live = there && lane * 4 + i < left;
+          if (live && kb != q8::kNanByte) emax = max(emax, kb);
+          if (live && vb != q8::kNanByte) vmax = max(vmax, vb);
+          if (lane * 4 + i < left && !there) miss |= 1u << i;
+          if (live && vb == q8::kNanByte) vnan |= 1u << i;
+        }
+        emax = __reduce_max_sync(0xffffffffu, emax);
+        vmax = __reduce_max_sync(0xffffffffu, vmax);
+        // the reference moves when the largest scale leaves fp16's range above it
+        if (vref < 0 || vmax > vref + kVHead) vref = max(vmax - kVHead, 0);
+        const bool special = __any_sync(0xffffffffu, (miss | vnan) != 0);
+        TileInfo& info = s_info[t % kInfo];
+        uint32_t kf[2] = {0, 0}, vf[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int kb = ksc >> (8 * i) & 0xff, vb = vsc >> (8 * i) & 0xff;
+          kf[i >> 1] |= (f16_pow2(min(kb - emax, 0)) & 0xffffu) << (16 * (i & 1));
+          vf[i >> 1] |= (vb == q8::kNanByte ? 0x7fffu : f16_pow2(min(vb - vref, kVHead)) & 0xffffu) << (16 * (i & 1));
+        }
+        *reinterpret_cast<uint2*>(info.kf + 4 * lane) = make_uint2(kf[0], kf[1]);
+        *reinterpret_cast<uint2*>(info.vf + 4 * lane) = make_uint2(vf[0], vf[1]);
+        if (lane == 0) {
+          info.scale = p.scale_log2 * q8::scale_of(emax);
+          info.vref = vref;
+          info.special = special;
+        }
+        if (special) {  // bits of tokens 4 lane .. + 3 into words of 32
+          miss <<= (lane & 7) * 4, vnan <<= (lane & 7) * 4;
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) {
+            miss |= __shfl_xor_sync(0xffffffffu, miss, o);
+            vnan |= __shfl_xor_sync(0xffffffffu, vnan, o);
+          }
+          if ((lane & 7) == 0) info.missing[lane >> 3] = miss, info.vnan[lane >> 3] = vnan;
+        }
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(info_full(t)) : "memory");
+        ksc = ksc_next, vsc = vsc_next;
+        if (t + 2 < n_tiles) ksc_next = fetch_scales(p.ks, t + 2), vsc_next = fetch_scales(p.vs, t + 2);
+      }
+    }
     bool ok = warp == kMmaWarp;
     for (int g = 0; ok && g < 2; ++g) {
       const int t = tile_at(g, 0);
@@ -460,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     const int g = warp / kGroupWarps;
     const int half = (warp % kGroupWarps) / 4, rq = warp % 4;
     const int row = rq * 32 + lane;  // of the group, and TMEM lane
-    const int r = rt.row0 + (p.alt ? 0 : g * kBM) + row;
+    const int r = rt.row0 + (ALT ? 0 : g * kBM) + row;
     const bool valid = r < rt.n_rows;
     const int tok = valid ? r / p.n_rep : 0;
     const int len = __ldg(p.lens + rt.b);
@@ -472,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     const uint32_t ts = t_s(g) + lane_base + sc0, to = t_o(g) + lane_base + oc0;
     const uint32_t bar_id = 2 + g * 4 + rq;  // the two warps that share these rows
     float* mxg = s_mx + g * 4 * kBM;
-    const float qf = s_qf[(p.alt ? 0 : g * kBM) + row];
+    const float qf = s_qf[(ALT ? 0 : g * kBM) + row];
     float m_ref = -INFINITY, l_run = 0.f;
     int vref = -1;  // reference of the values in O
     bool failed = false, row_nan = false;
@@ -614,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     const int vexp = vref - 127;
     const int64_t o = static_cast<int64_t>(rt.q0 + tok) * p.Hq + hkv * p.n_rep + (valid ? r % p.n_rep : 0);
     const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
-    const int part = p.alt ? 2 * split + g : split;
+    const int part = ALT ? 2 * split + g : split;
     if (all_ok && k > 0) tc::tc_fence_after();
 #pragma unroll
     for (int c0 = 0; c0 < kOC; c0 += 32) {
@@ -696,20 +745,28 @@ __global__ void __launch_bounds__(256) chunk_q8_merge_kernel(const __grid_consta
   if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = nan ? inv : M == -INFINITY ? -INFINITY : M + logf(W);
 }
 
-template <typename T, int D>
-int launch(const ChunkQ8Params& p, cudaStream_t st) {
-  auto kern = chunk_q8_kernel<T, D>;
+template <typename T, int D, bool ALT>
+int launch_chunk(const ChunkQ8Params& p, cudaStream_t st) {
+  auto kern = chunk_q8_kernel<T, D, ALT>;
+  constexpr int kBytes = Layout<D, ALT>::kBytes;
   static bool raised[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !raised[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes) != cudaSuccess) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) {
       set_error("q8_attention_launch:smem_attr");
       return BPKV_ERR_CUDA;
     }
     if (dev >= 0 && dev < 64) raised[dev] = true;
   }
-  kern<<<static_cast<unsigned>(p.B * p.tiles * p.splits * p.Hkv), kThreads, Layout<D>::kBytes, st>>>(p);
+  kern<<<static_cast<unsigned>(p.B * p.tiles * p.splits * p.Hkv), kThreads, kBytes, st>>>(p);
+  return BPKV_OK;
+}
+
+template <typename T, int D>
+int launch(const ChunkQ8Params& p, cudaStream_t st) {
+  const int rc = p.alt ? launch_chunk<T, D, true>(p, st) : launch_chunk<T, D, false>(p, st);
+  if (rc != BPKV_OK) return rc;
   if (p.parts > 1) {
     const int64_t rows = static_cast<int64_t>(p.total_q) * p.Hq;
     const cudaError_t e = launch_pdl(chunk_q8_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, p);

@@ -144,14 +144,24 @@ __device__ __forceinline__ int find_item(const int* prefix, int n, int s) {
   }
   return lo;
 }
-__device__ __forceinline__ int range_at(int c, int total, int W) {
-  return static_cast<int>(static_cast<int64_t>(c) * total / W);
-}
+// Equal shares of `total` pages for W workers: the first total % W take one more.  With fewer pages than
+// workers the first `total` workers have a page each.
+struct Shares {
+  int per, more;
+  __device__ __forceinline__ Shares(int total, int W) : per(total / W), more(total % W) {}
+  __device__ __forceinline__ int start(int c) const { return c * per + min(c, more); }
+  __device__ __forceinline__ int owner(int page) const {
+    const int big = more * (per + 1);
+    return page < big ? page / (per + 1) : more + (page - big) / per;  // per > 0 where a page lies past `big`
+  }
+};
 
 // A worker's walk over its pages: item by item, pages [page, end) of each.
 template <int R>
 struct Walk {
   int item, page, end, next;  // next: first flattened page not yet visited (split), or next item (not split)
+  int tokens, page_id;        // of the item; of its page `page` (loader only)
+  const int32_t* bt_row;
   __device__ __forceinline__ bool live() const { return item >= 0; }
 };
 template <int R>
@@ -216,6 +226,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   constexpr int CH = D / 16;              // 16-byte pieces per row
   constexpr int KS = D / 16;              // MMA k-steps of S
   constexpr int MT = D / 16;              // 16-row tiles of O^T
+  constexpr bool kEarlyV = NT <= 2;       // V codes into registers before the softmax, which hides their latency
 
   int* prefix = reinterpret_cast<int*>(smem + NW * NS * STAGEB);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -241,31 +252,36 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   const int h = blockIdx.y * p.hp + warp % p.hp;
   const int worker = blockIdx.x * p.pl + warp / p.hp;
   if (warp / p.hp >= p.pl || h >= p.Hkv) return;
-  const int total = p.split ? prefix[p.n_items] : 0;
-  const int s_beg = p.split ? range_at(worker, total, W) : 0, s_end = p.split ? range_at(worker + 1, total, W) : 0;
+  int s_beg = 0, s_end = 0;
+  if (p.split) {
+    const Shares sh(prefix[p.n_items], W);
+    s_beg = sh.start(worker), s_end = sh.start(worker + 1);
+  }
 
   const uint32_t ring = smem_u32(smem + warp * NS * STAGEB);
   const int g = lane >> 2, c = lane & 3;
 
   // ---- loader: one page of this head into a ring stage ----
+  const int64_t row_stride = static_cast<int64_t>(p.Hkv) * D;
+  // this lane's pieces are ch0 of rows tok0, tok0 + 32 / CH, ...
+  const int tok0 = lane / CH, ch0 = lane % CH;
+  const int64_t lane_off = static_cast<int64_t>(h) * D + tok0 * row_stride + ch0 * 16;
   auto issue = [&](const Walk<R>& w, int stage) {
-    const Item it = item_of<R>(p, w.item);
-    const int page = q8::page_of(p.bt + static_cast<int64_t>(it.b) * p.bt_sb, w.page, p.max_blocks, p.num_pages);
+    const int page = w.page_id;
     // rows past the item's last visible token are zero-filled, so that what a page holds there never
     // reaches the MMAs
-    const int live = page < 0 ? 0 : min(kPage, item_tokens<R>(p, it) - w.page * kPage);
-    const uint8_t* kp = p.kc + (page < 0 ? 0 : page * p.page_stride + static_cast<int64_t>(h) * D);
-    const uint8_t* vp = p.vc + (page < 0 ? 0 : page * p.page_stride + static_cast<int64_t>(h) * D);
+    const int live = page < 0 ? 0 : min(kPage, w.tokens - w.page * kPage);
+    const int64_t off = page < 0 ? 0 : page * p.page_stride + lane_off;
+    const uint8_t *kp = p.kc + off, *vp = p.vc + off;
     const uint32_t sk = ring + stage * STAGEB;
 #pragma unroll
     for (int r = 0; r < CH / 2; ++r) {
-      const int ci = lane + 32 * r;
-      const int tok = ci / CH, ch = ci % CH;
+      const int tok = tok0 + r * (32 / CH);
       const bool ok = tok < live;
-      const int64_t off = ok ? static_cast<int64_t>(tok) * p.Hkv * D + ch * 16 : 0;
-      const uint32_t so = piece<D>(tok, ch);
-      cp_async16(sk + so, kp + off, ok);
-      cp_async16(sk + TILEB + so, vp + off, ok);
+      const int64_t o = ok ? r * (32 / CH) * row_stride : 0;
+      const uint32_t so = piece<D>(tok, ch0);
+      cp_async16(sk + so, kp + o, ok);
+      cp_async16(sk + TILEB + so, vp + o, ok);
     }
     if (lane < 2) {
       const uint8_t* sp = (lane == 0 ? p.ks : p.vs) + (page < 0 ? 0 : page * p.scale_stride + h * kPage);
@@ -279,11 +295,22 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   ld.item = cs.item = -1;
   ld.page = cs.page = ld.end = cs.end = 0;
   ld.next = cs.next = p.split ? s_beg : worker;
-  walk_next<R>(p, prefix, worker, W, s_end, ld);
+  auto load_seek = [&]() {  // the loader's next item
+    walk_next<R>(p, prefix, worker, W, s_end, ld);
+    if (ld.live()) {
+      const Item it = item_of<R>(p, ld.item);
+      ld.tokens = item_tokens<R>(p, it);
+      ld.bt_row = p.bt + static_cast<int64_t>(it.b) * p.bt_sb;
+      ld.page_id = q8::page_of(ld.bt_row, ld.page, p.max_blocks, p.num_pages);
+    }
+  };
+  load_seek();
   auto load_one = [&](int stage) {
     if (ld.live()) {
       issue(ld, stage);
-      if (++ld.page == ld.end) walk_next<R>(p, prefix, worker, W, s_end, ld);
+      // the next page's id is fetched now, to be there when its turn comes
+      if (++ld.page == ld.end) load_seek();
+      else ld.page_id = q8::page_of(ld.bt_row, ld.page, p.max_blocks, p.num_pages);
     }
     cp_async_commit();
   };
@@ -362,31 +389,55 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       int live;
       asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(live) : "r"(ss + 32));
       const int t0 = cs.page * kPage;
-      // ---- S^T = K Q^T: rows tokens g, g + 8; columns query rows ----
-      float s[NT][4];
+      // V codes: lane (mi, row) of ldmatrix addresses token (row + 8 (mi & 1)), piece mt + (mi >> 1)
+      auto load_v = [&](int mt, uint32_t* r) {
+        const int tok = (lane & 7) + 8 * ((lane >> 3) & 1);
+        ldmatrix_x4_trans(sv + piece<D>(tok, mt + (lane >> 4)), r[0], r[1], r[2], r[3]);
+      };
+      uint32_t vr[kEarlyV ? MT / 2 : 1][4];
+      if constexpr (kEarlyV) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < CH / 4; ++j) {
-        const int ch = D == 64 ? c : 2 * c + (j & 1) + 8 * (j >> 1);
-        const uint4 ka = lds128(sk + piece<D>(g, ch)), kb = lds128(sk + piece<D>(g + 8, ch));
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t a[4];
-          q8::e4m3x4_to_f16x4(wa[w], a[0], a[2]);
-          q8::e4m3x4_to_f16x4(wb[w], a[1], a[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<__half>(s[nt], a, qb[nt][4 * j + w][0], qb[nt][4 * j + w][1]);
-        }
+        for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
       }
-      // ---- scores, online softmax in log2 ----
       const bool ok0 = g < live, ok1 = g + 8 < live;
       const int kb0 = lds_u8(ss + g), kb1 = lds_u8(ss + g + 8);
       int vb0 = ok0 ? lds_u8(ss + 16 + g) : 0, vb1 = ok1 ? lds_u8(ss + 16 + g + 8) : 0;
+      // ---- S^T = K Q^T: rows tokens g, g + 8; columns query rows; two chains of MMAs ----
+      float s[NT][4];
+      {
+        float s2[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < CH / 4; ++j) {
+          const int ch = D == 64 ? c : 2 * c + (j & 1) + 8 * (j >> 1);
+          const uint4 ka = lds128(sk + piece<D>(g, ch)), kb = lds128(sk + piece<D>(g + 8, ch));
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t a[4];
+            q8::e4m3x4_to_f16x4(wa[w], a[0], a[2]);
+            q8::e4m3x4_to_f16x4(wb[w], a[1], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<__half>(NT <= 2 && (w & 1) ? s2[nt] : s[nt], a, qb[nt][4 * j + w][0], qb[nt][4 * j + w][1]);
+          }
+        }
+        if constexpr (NT <= 2) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
+        }
+      }
+      // ---- scores, online softmax in log2 ----
       const float kf0 = q8::scale_of(kb0), kf1 = q8::scale_of(kb1);
       const bool edge = live < kPage || t0 + kPage - 1 > lim_min;
-      bool grow = false;
+      // Rare, and looked for with one vote: a row whose maximum outgrew its reference, a value scale above
+      // the reference so far, a value row that is not finite.
+      bool rare = max(vb0, vb1) > vref || vb0 == q8::kNanByte || vb1 == q8::kNanByte;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -397,10 +448,10 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
             s[nt][e] = (ok0 && t0 + g <= lim[nt][e]) ? s[nt][e] : -INFINITY;
             s[nt][2 + e] = (ok1 && t0 + g + 8 <= lim[nt][e]) ? s[nt][2 + e] : -INFINITY;
           }
-          grow |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + kMaxLazy;
+          rare |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + kMaxLazy;
         }
       }
-      if (__any_sync(0xffffffffu, grow)) {
+      if (__any_sync(0xffffffffu, rare)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -420,42 +471,46 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
             }
           }
         }
-      }
-      // a value row that is not finite: its codes are taken out, and the rows that see it become NaN
-      if (__any_sync(0xffffffffu, vb0 == q8::kNanByte || vb1 == q8::kNanByte)) {
+        // a value row that is not finite: its codes are taken out, and the rows that see it become NaN
+        if (__any_sync(0xffffffffu, vb0 == q8::kNanByte || vb1 == q8::kNanByte)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+          for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            bool bad = (vb0 == q8::kNanByte && s[nt][e] != -INFINITY) || (vb1 == q8::kNanByte && s[nt][2 + e] != -INFINITY);
-            uint32_t who = __ballot_sync(0xffffffffu, bad);
-            who |= who >> 16, who |= who >> 8, who |= who >> 4;
-            if (who >> c & 1) {
+            for (int e = 0; e < 2; ++e) {
+              bool bad = (vb0 == q8::kNanByte && s[nt][e] != -INFINITY) || (vb1 == q8::kNanByte && s[nt][2 + e] != -INFINITY);
+              uint32_t who = __ballot_sync(0xffffffffu, bad);
+              who |= who >> 16, who |= who >> 8, who |= who >> 4;
+              if (who >> c & 1) {
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) acc[nt][mt][e] = acc[nt][mt][2 + e] = __int_as_float(0x7fc00000);
+                for (int mt = 0; mt < MT; ++mt) acc[nt][mt][e] = acc[nt][mt][2 + e] = __int_as_float(0x7fc00000);
+              }
             }
           }
+          for (int t = 0; t < kPage; ++t) {
+            const bool bad = t < live && lds_u8(ss + 16 + t) == q8::kNanByte;
+            if (bad && lane < CH)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(sv + piece<D>(t, lane)), "r"(0) : "memory");
+          }
+          if (vb0 == q8::kNanByte) vb0 = 0;
+          if (vb1 == q8::kNanByte) vb1 = 0;
+          __syncwarp();
+          if constexpr (kEarlyV) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
+          }
         }
-        for (int t = 0; t < kPage; ++t) {
-          const bool bad = t < live && lds_u8(ss + 16 + t) == q8::kNanByte;
-          if (bad && lane < CH)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(sv + piece<D>(t, lane)), "r"(0) : "memory");
+        const int vmax = __reduce_max_sync(0xffffffffu, max(vb0, vb1));
+        if (vmax > vref) {
+          // 2^(vref - vmax); far below: nothing of the old sum is left
+          const float a = vmax - vref > 126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - (vmax - vref)) << 23);
+          vref = vmax;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nt][mt][e] *= a;
         }
-        if (vb0 == q8::kNanByte) vb0 = 0;
-        if (vb1 == q8::kNanByte) vb1 = 0;
-        __syncwarp();
-      }
-      const int vmax = __reduce_max_sync(0xffffffffu, max(vb0, vb1));
-      if (vmax > vref) {
-        // 2^(vref - vmax); far below: nothing of the old sum is left
-        const float a = vmax - vref > 126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - (vmax - vref)) << 23);
-        vref = vmax;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][mt][e] *= a;
       }
       const int ve0 = vb0 - vref + kWOff + 127, ve1 = vb1 - vref + kWOff + 127;
       const float vf0 = ve0 > 0 ? __uint_as_float(static_cast<uint32_t>(ve0) << 23) : 0.f;
@@ -486,23 +541,21 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         pb[nt][1] = movmatrix_trans(pb[nt][1]);
       }
       // ---- O^T += V^T P^T ----
-      {
-        const int mi = lane >> 3, tok = (lane & 7) + 8 * (mi & 1);
 #pragma unroll
-        for (int mt = 0; mt < MT; mt += 2) {
-          uint32_t r[4];
-          ldmatrix_x4_trans(sv + piece<D>(tok, mt + (mi >> 1)), r[0], r[1], r[2], r[3]);
+      for (int mt = 0; mt < MT; mt += 2) {
+        uint32_t late[4];
+        if constexpr (!kEarlyV) load_v(mt, late);
+        const uint32_t* r = kEarlyV ? vr[kEarlyV ? mt / 2 : 0] : late;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            // bytes (token 2c: d, d + 1; token 2c + 1: d, d + 1) -> (d: both tokens), (d + 1: both tokens)
-            uint32_t a[4];
-            q8::e4m3x4_to_f16x4(__byte_perm(r[2 * u], 0, 0x3120), a[0], a[1]);
-            q8::e4m3x4_to_f16x4(__byte_perm(r[2 * u + 1], 0, 0x3120), a[2], a[3]);
+        for (int u = 0; u < 2; ++u) {
+          // bytes (token 2c: d, d + 1; token 2c + 1: d, d + 1) -> (d: both tokens), (d + 1: both tokens)
+          uint32_t a[4];
+          q8::e4m3x4_to_f16x4(__byte_perm(r[2 * u], 0, 0x3120), a[0], a[1]);
+          q8::e4m3x4_to_f16x4(__byte_perm(r[2 * u + 1], 0, 0x3120), a[2], a[3]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<__half>(acc[nt][mt + u], a, pb[nt][0], pb[nt][1]);
-              if constexpr (kTwoParts) mma16816<__half>(acc[nt][mt + u], a, pl[nt][0], pl[nt][1]);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<__half>(acc[nt][mt + u], a, pb[nt][0], pb[nt][1]);
+            if constexpr (kTwoParts) mma16816<__half>(acc[nt][mt + u], a, pl[nt][0], pl[nt][1]);
           }
         }
       }
@@ -554,92 +607,97 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
 
 // Merges the items that several workers share.  CTA = (unit, one query row); a unit is an
 // item when there are no more items than workers, otherwise the boundary between workers
-// u and u + 1.  Warp w of 8 sums parts w, w + 8, ...; a lane holds D / 32 columns.
-constexpr int kCombWarps = 8;
+// u and u + 1.  The weights of the parts are formed once in shared memory; warp w then
+// sums parts w, w + warps, ...; a lane holds D / 32 columns.  The launch takes as many
+// warps as an item has parts on average.
+constexpr int kCombMaxWarps = 32;
+constexpr int kMaxWorkers = 2560;  // parts of one item: their weights fit in shared memory
 
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(kCombWarps * 32) q8_combine_kernel(Q8Params p, int W, int by_item) {
-  __shared__ int s_find[3];
-  __shared__ float s_red[2][kCombWarps];
-  __shared__ float s_acc[kCombWarps][D];
+__global__ void __launch_bounds__(kCombMaxWarps * 32) q8_combine_kernel(Q8Params p, int W, int by_item) {
+  extern __shared__ float s_w[];  // [parts], at most W
+  __shared__ float s_red[kCombMaxWarps];
+  __shared__ float s_acc[kCombMaxWarps][D];
   constexpr int C = D / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int total = p.g_prefix[p.n_items];
   if (total == 0) return;
+  const Shares sh(total, W);
   int item = blockIdx.x;
   if (!by_item) {
-    const int s = range_at(blockIdx.x + 1, total, W);
-    if (s >= total || range_at(blockIdx.x, total, W) == s) return;
-    if (tid == 0) {
-      s_find[0] = find_item(p.g_prefix, p.n_items, s);
-    }
-    __syncthreads();
-    item = s_find[0];
-    // this boundary is the item's first one (earlier boundaries lie at or before its first page)
+    const int s = sh.start(blockIdx.x + 1);
+    if (s >= total) return;
+    item = find_item(p.g_prefix, p.n_items, s);
+    // this boundary is the item's first one: worker blockIdx.x has its first page
     const int first0 = p.g_prefix[item];
-    if (first0 >= s || range_at(blockIdx.x, total, W) > first0) return;
+    if (first0 >= s || sh.start(blockIdx.x) > first0) return;
   }
   const int first = p.g_prefix[item], last = p.g_prefix[item + 1];
   if (first == last) return;  // written by the attention kernel
-  const int c_lo = static_cast<int>(((static_cast<int64_t>(first) + 1) * W - 1) / total);
-  const int c_hi = static_cast<int>((static_cast<int64_t>(last) * W - 1) / total);
-  if (c_lo == c_hi) return;  // one worker had all of it
+  const int c_lo = sh.owner(first), n = sh.owner(last - 1) - c_lo + 1;
+  if (n == 1) return;  // one worker had all of it
   const int h = blockIdx.y / p.rows_max, rl = blockIdx.y % p.rows_max;
   const Item it = item_of<R>(p, item);
   const int r = it.row0 + rl;
   if (r >= it.n_rows) return;
-  // part of worker w; -1 where it has no pages
-  auto part = [&](int w) -> int64_t {
-    const int s = range_at(w, total, W);
-    if (range_at(w + 1, total, W) == s) return -1;
-    return (static_cast<int64_t>(2 * w + (s >= first ? 0 : 1)) * p.Hkv + h) * R + rl;
-  };
-  // a worker's first segment is slot 0: the item begins there exactly when s == first
-  float M = -INFINITY;
-  for (int w = c_lo + tid; w <= c_hi; w += blockDim.x) {
-    const int64_t i = part(w);
-    if (i >= 0) {
-      const float x = p.part_lse[i];
-      M = (x != x || M != M) ? __int_as_float(0x7fc00000) : fmaxf(M, x);
-    }
+  // The item is the last one of worker c_lo (slot 1, or slot 0 if that worker begins with it) and the
+  // first one of the workers after it (slot 0).
+  const int64_t step = 2 * static_cast<int64_t>(p.Hkv) * R;
+  const int64_t part0 = (static_cast<int64_t>(2 * c_lo) * p.Hkv + h) * R + rl;
+  const int64_t lead = sh.start(c_lo) < first ? static_cast<int64_t>(p.Hkv) * R : 0;
+  auto part = [&](int i) { return part0 + i * step + (i == 0 ? lead : 0); };
+  const float nan = __int_as_float(0x7fc00000);
+  float M = -INFINITY;  // NaN once any part is (fmaxf alone would drop it)
+  for (int i = tid; i < n; i += blockDim.x) {
+    const float x = p.part_lse[part(i)];
+    s_w[i] = x;
+    M = (x != x || M != M) ? nan : fmaxf(M, x);
   }
   for (int o = 16; o > 0; o >>= 1) {
     const float x = __shfl_xor_sync(0xffffffffu, M, o);
-    M = (x != x || M != M) ? __int_as_float(0x7fc00000) : fmaxf(M, x);
+    M = (x != x || M != M) ? nan : fmaxf(M, x);
   }
-  if (lane == 0) s_red[0][warp] = M;
+  if (lane == 0) s_red[warp] = M;
   __syncthreads();
-  M = s_red[0][0];
-  for (int w = 1; w < kCombWarps; ++w) {
-    const float x = s_red[0][w];
-    M = (x != x || M != M) ? __int_as_float(0x7fc00000) : fmaxf(M, x);
+  M = s_red[0];
+  for (int w = 1; w < nw; ++w) {
+    const float x = s_red[w];
+    M = (x != x || M != M) ? nan : fmaxf(M, x);
   }
-  float a[C] = {}, L = 0.f;
-  if (M != -INFINITY) {
-#pragma unroll 4
-    for (int w = c_lo + warp; w <= c_hi; w += kCombWarps) {
-      const int64_t i = part(w);
-      if (i < 0) continue;
-      const float x = p.part_lse[i];
-      if (x == -INFINITY) continue;
-      const float wt = exp2f((x - M) * 1.4426950408889634f);
-      L += wt;
-      const float* src = p.part_o + i * D + lane * C;
+  __syncthreads();
+  float L = 0.f;
+  for (int i = tid; i < n; i += blockDim.x) {
+    const float w = M == -INFINITY ? 0.f : exp2f((s_w[i] - M) * 1.4426950408889634f);
+    s_w[i] = w;
+    L += w;
+  }
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  if (lane == 0) s_red[warp] = L;
+  __syncthreads();
+  L = 0.f;
+  for (int w = 0; w < nw; ++w) L += s_red[w];
+  float a[C] = {};
+#pragma unroll 8
+  for (int i = warp; i < n; i += nw) {
+    const float w = s_w[i];
+    const float* src = p.part_o + part(i) * D + lane * C;
+    float x[C];
+    if constexpr (C == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+    else
 #pragma unroll
-      for (int k = 0; k < C; ++k) a[k] += wt * src[k];
-    }
+      for (int k = 0; k < C; k += 4) *reinterpret_cast<float4*>(x + k) = *reinterpret_cast<const float4*>(src + k);
+    // a part of a worker that saw none of its tokens (w = 0) holds zeros; NaN parts stay NaN
+#pragma unroll
+    for (int k = 0; k < C; ++k) a[k] += w * x[k];
   }
 #pragma unroll
   for (int k = 0; k < C; ++k) s_acc[warp][lane * C + k] = a[k];
-  if (lane == 0) s_red[1][warp] = L;
   __syncthreads();
-  L = 0.f;
-  for (int w = 0; w < kCombWarps; ++w) L += s_red[1][w];
   const int64_t o = static_cast<int64_t>(it.q0 + r / p.n_rep) * p.Hq + h * p.n_rep + r % p.n_rep;
   for (int d = tid; d < D; d += blockDim.x) {
     float y = 0.f;
-    for (int w = 0; w < kCombWarps; ++w) y += s_acc[w][d];
+    for (int w = 0; w < nw; ++w) y += s_acc[w][d];
     static_cast<T*>(p.out)[o * D + d] = Elem<T>::from_f(M == -INFINITY ? p.empty : y / L);
   }
   if (tid == 0 && p.lse_out != nullptr) p.lse_out[o] = M == -INFINITY ? -INFINITY : M + logf(L);
@@ -691,7 +749,7 @@ Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max
   pl.hp = (Hkv + pl.groups - 1) / pl.groups;
   pl.pl = pl.nw / pl.hp;
   const int sms = sm_count();
-  pl.grid = sms / pl.groups > 0 ? sms / pl.groups : 1;
+  pl.grid = max(1, min(sms / pl.groups, kMaxWorkers / pl.pl));
   const int64_t tiles = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
   const int64_t items = tiles * B;
   pl.tiles = static_cast<int>(tiles);
@@ -729,7 +787,12 @@ int launch_attend(Q8Params& p, const Plan& pl, cudaStream_t st) {
     const int by_item = pl.n_items <= W;
     const dim3 grid(by_item ? pl.n_items : W - 1, p.Hkv * p.rows_max);
     if (W > 1) {
-      const cudaError_t e = launch_pdl(q8_combine_kernel<T, D, 8 * NT>, grid, dim3(kCombWarps * 32), 0, st, p, W, by_item);
+      // about as many warps as an item has parts, 2 to 32, but no more than the SMs hold at once
+      int warps = 2;
+      while (warps < kCombMaxWarps && static_cast<int64_t>(warps) * pl.n_items < W &&
+             static_cast<int64_t>(2 * warps) * grid.x * grid.y <= 64LL * sm_count())
+        warps *= 2;
+      const cudaError_t e = launch_pdl(q8_combine_kernel<T, D, 8 * NT>, grid, dim3(warps * 32), sizeof(float) * W, st, p, W, by_item);
       if (e != cudaSuccess) {
         set_error("q8_attention_launch:%s", cudaGetErrorString(e));
         return BPKV_ERR_CUDA;

@@ -41,15 +41,11 @@ __device__ __forceinline__ uint32_t to_e4m3x2(float a, float b) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }
-// Two e4m3 codes -> fp16 pair (low byte in the low half).  Exact: 4 significant bits, 2^-9..448.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"(c));
-  return r;
-}
+// Four e4m3 codes -> fp16, bytes 0 and 1 in `lo`, 2 and 3 in `hi`.  Exact: 4 significant bits, 2^-9..448.
 __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  lo = e4m3x2_to_f16x2(static_cast<uint16_t>(w & 0xffffu));
-  hi = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 
 // Page of request row `bt_row`, logical index j; -1 where the table has no such

@@ -43,6 +43,11 @@ from .pool import PagedKVPool
 
 HEAD_DIMS = (64, 128, 256)
 
+# the current device and stream handle without building Python objects: a call's host time is what a short one takes
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_stream = (torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream")
+           else lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 class QuantPagedKV(NamedTuple):
     """One layer of an 8-bit paged cache (views are fine: only a page has to be dense)."""
@@ -55,16 +60,17 @@ class QuantPagedKV(NamedTuple):
 def _check_kv(kv: QuantPagedKV, what: str) -> Tuple[int, int, int]:
     """Sizes (pages, kv_heads, head_dim) of a well-formed layer."""
     kc, vc, ks, vs = kv
-    if kc.dim() != 4 or vc.shape != kc.shape:
+    shape, scales = kc.shape, ks.shape
+    if len(shape) != 4 or vc.shape != shape:
         raise RuntimeError(f"{what}_shape_unsupported:cache_rank")
-    n, page, h_kv, d = kc.shape
+    n, page, h_kv, d = shape
     if page != 16:
         raise RuntimeError(f"{what}_shape_unsupported:block_size_{page}")
     if d not in HEAD_DIMS:
         raise RuntimeError(f"{what}_shape_unsupported:head_dim_{d}")
-    if kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
+    if kc.dtype is not torch.float8_e4m3fn or vc.dtype is not torch.float8_e4m3fn:
         raise RuntimeError(f"{what}_shape_unsupported:cache_dtype")
-    if ks.shape != (n, h_kv, 16) or vs.shape != ks.shape or ks.dtype != torch.uint8 or vs.dtype != torch.uint8:
+    if scales != (n, h_kv, 16) or vs.shape != scales or ks.dtype is not torch.uint8 or vs.dtype is not torch.uint8:
         raise RuntimeError(f"{what}_shape_unsupported:scales")
     s, t = kc.stride(), ks.stride()
     if s[3] != 1 or (s[2] != d and h_kv > 1) or s[1] != h_kv * d or vc.stride() != s:
@@ -137,7 +143,7 @@ def quantize_append(kv: QuantPagedKV, k_new: torch.Tensor, v_new: torch.Tensor, 
     cu = None if cu_seqlens_q is None else _int32(cu_seqlens_q, what, "cu_seqlens", B + 1)
     dev = k_new.device
     _check_device(what, dev, *kv, v_new, bt, lens, cu)
-    if dev.index != torch.cuda.current_device():  # the library launches on the current device
+    if dev.index != _device():  # the library launches on the current device
         with torch.cuda.device(dev):
             return quantize_append(kv, k_new, v_new, bt, lens, cu)
     k, v = _aligned(k_new), _aligned(v_new)
@@ -146,7 +152,7 @@ def quantize_append(kv: QuantPagedKV, k_new: torch.Tensor, v_new: torch.Tensor, 
         k.data_ptr(), v.data_ptr(), kv.k_codes.data_ptr(), kv.v_codes.data_ptr(), kv.k_scales.data_ptr(),
         kv.v_scales.data_ptr(), bt.data_ptr(), _lib.ptr(cu), lens.data_ptr(), B, total, h_kv, d, bt.shape[1], n,
         ks[0], ks[1], vs[0], vs[1], kv.k_codes.stride(0), kv.k_scales.stride(0), bt.stride(0), code,
-        torch.cuda.current_stream(dev).cuda_stream)
+        _stream(dev.index))
     if rc:
         _lib.check(rc, what)
 
@@ -188,14 +194,14 @@ def dequantize_pages(kv: QuantPagedKV, block_table: torch.Tensor, cu_seqlens: to
         if s[2] != 1 or s[0] % per or s[1] % per or v.stride() != s or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise RuntimeError(f"{what}_shape_unsupported:out_layout")
     _check_device(what, dev, *kv, bt, cu, st, k, v)
-    if dev.index != torch.cuda.current_device():  # the library launches on the current device
+    if dev.index != _device():  # the library launches on the current device
         with torch.cuda.device(dev):
             return dequantize_pages(kv, bt, cu, total, starts=st, out=(k, v))
     rc = lib.bpkv_q8_dequantize(
         kv.k_codes.data_ptr(), kv.v_codes.data_ptr(), kv.k_scales.data_ptr(), kv.v_scales.data_ptr(), bt.data_ptr(),
         cu.data_ptr(), _lib.ptr(st), k.data_ptr(), v.data_ptr(), B, total, h_kv, d, bt.shape[1], n,
         kv.k_codes.stride(0), kv.k_scales.stride(0), bt.stride(0), k.stride(0), k.stride(1), code,
-        torch.cuda.current_stream(dev).cuda_stream)
+        _stream(dev.index))
     if rc:
         _lib.check(rc, what)
     return k, v
@@ -225,7 +231,7 @@ def _attention(what: str, q: torch.Tensor, kv: QuantPagedKV, block_table: torch.
         raise RuntimeError(f"{what}_shape_unsupported:lse_out")
     dev = q.device
     _check_device(what, dev, *kv, bt, lens, cu, lse_out)
-    if dev.index != torch.cuda.current_device():  # the library launches on the current device
+    if dev.index != _device():  # the library launches on the current device
         with torch.cuda.device(dev):
             return _attention(what, q, kv, bt, lens, cu, max_q, softmax_scale, n_rep, causal, lse_out)
     q = _aligned(q)
@@ -237,7 +243,7 @@ def _attention(what: str, q: torch.Tensor, kv: QuantPagedKV, block_table: torch.
         q.data_ptr(), kv.k_codes.data_ptr(), kv.v_codes.data_ptr(), kv.k_scales.data_ptr(), kv.v_scales.data_ptr(),
         bt.data_ptr(), _lib.ptr(cu), lens.data_ptr(), out.data_ptr(), _lib.ptr(lse_out), B, total, h_q, h_kv, d, bt.shape[1],
         n, max_q, qs[0], qs[1], kv.k_codes.stride(0), kv.k_scales.stride(0), bt.stride(0), float(softmax_scale),
-        int(causal), int(cu is None), code, _lib.ptr(ws), ws_bytes, torch.cuda.current_stream(dev).cuda_stream)
+        int(causal), int(cu is None), code, _lib.ptr(ws), ws_bytes, _stream(dev.index))
     if rc:
         _lib.check(rc, what)
     return out
