@@ -12,17 +12,21 @@ struct ChunkQ8Params {
   const uint8_t* ks;
   const uint8_t* vs;
   const int32_t* bt;
-  const int32_t* cu_q;
+  const int32_t* cu_q;  // null: request b has the one query row b
   const int32_t* lens;
   void* out;
   float* lse_out;
   float* part_o;    // [parts][total_q * Hq][D]
   float* part_lse;  // [parts][total_q * Hq]
-  int B, Hq, Hkv, n_rep, tiles, splits, parts, alt, causal, max_blocks, num_pages, total_q;
+  int B, Hq, Hkv, n_rep, tiles, splits, parts, alt, ranked, causal, max_blocks, num_pages, total_q;
+  // ranked: the row tiles are taken longest first, each CTA working the order out (at most kMaxRanked of them)
   int64_t q_st, q_sh, page_stride, scale_stride, bt_sb;
   float scale_log2;
+  float empty;  // value of a row that sees no token
 };
 
+constexpr int kMaxRanked = 512;
+constexpr int kMaxParts = 64;  // of a row; a multiple of 32
 // head_dim 64 or 128, softmax scale > 0.
 int chunk_q8_tc_launch(const ChunkQ8Params& p, int head_dim, int dtype, cudaStream_t st);
 

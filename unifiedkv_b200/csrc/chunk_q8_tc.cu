@@ -52,7 +52,6 @@ constexpr int kThreads = 28 * 32;
 constexpr int kRegsSoftmax = 88, kRegsConv = 56, kRegsMma = 40;
 static_assert(128 * (4 * kRegsSoftmax + 2 * kRegsConv + kRegsMma) <= kThreads * 72, "register split");
 constexpr int kMaxPages = 1024;       // block-table entries staged in shared memory
-constexpr int kMaxRanked = 512;       // row tiles ordered longest first
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescale = 4.f, kWOff = 11.f;  // weights <= 2^4, held times 2^11
 constexpr int kVHead = 6;                      // values are held as code * 2^(byte - vref), byte <= vref + 6
@@ -100,6 +99,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+// 32 bytes to a 32-byte boundary: a whole sector, where two 16-byte stores would write it in halves.
+__device__ __forceinline__ void stg256(void* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
@@ -143,8 +148,8 @@ __device__ __forceinline__ RowTile row_tile(const ChunkQ8Params& p, int i) {
   const int rows = ALT ? kBM : 2 * kBM;
   r.b = i / p.tiles;
   r.row0 = (i % p.tiles) * rows;
-  r.q0 = __ldg(p.cu_q + r.b);
-  r.n_q = __ldg(p.cu_q + r.b + 1) - r.q0;
+  r.q0 = p.cu_q == nullptr ? r.b : __ldg(p.cu_q + r.b);
+  r.n_q = p.cu_q == nullptr ? 1 : __ldg(p.cu_q + r.b + 1) - r.q0;
   r.n_rows = r.n_q * p.n_rep;
   const int len = __ldg(p.lens + r.b);
   r.kv_end = 0;
@@ -163,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t qs = smem_u32(smem), ks = qs + L::kQTiles * L::kQ, vs = ks + kRing * L::kKV;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  constexpr int kBarCount = 4 * kRing + 6 + 2 * kInfo;
+  constexpr int kBarCount = 4 * kRing + 7 + 2 * kInfo;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBarCount);
   static_assert((kBarCount + 1) * 8 <= 256, "barrier area");
   TileInfo* s_info = reinterpret_cast<TileInfo*>(smem + L::kInfoOff);
@@ -179,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   const int hkv = static_cast<int>(blockIdx.x % p.Hkv);
   const int split = static_cast<int>(blockIdx.x / p.Hkv) % p.splits;
   int item = static_cast<int>(blockIdx.x / p.Hkv) / p.splits;
-  if (n_items <= kMaxRanked) {
+  if (p.ranked) {
     __shared__ int s_item;
     for (int i = tid; i < n_items; i += kThreads) s_pages[i] = row_tile<ALT>(p, i).kv_end;
     __syncthreads();
@@ -191,7 +196,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     }
     __syncthreads();
     item = s_item;
-    __syncthreads();  // s_pages is about to be filled
   }
   const RowTile rt = row_tile<ALT>(p, item);
   if (rt.row0 >= rt.n_rows) return;  // uniform across the CTA, before any barrier or TMEM use
@@ -207,6 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   auto s_full = [&](int g) { return smem_u32(&bars[4 * kRing + g]); };
   auto p_full = [&](int g) { return smem_u32(&bars[4 * kRing + 2 + g]); };
   auto o_done = [&](int g) { return smem_u32(&bars[4 * kRing + 4 + g]); };
+  const uint32_t q_full = smem_u32(&bars[kBarCount - 1]);
   auto info_full = [&](int t) { return smem_u32(&bars[4 * kRing + 6 + t % kInfo]); };
   auto info_free = [&](int t) { return smem_u32(&bars[4 * kRing + 6 + kInfo + t % kInfo]); };
 
@@ -225,6 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       tc::mbar_init(info_full(i), 32u);
       tc::mbar_init(info_free(i), 1u);
     }
+    tc::mbar_init(q_full, 32u * 2 * kGroupWarps);
     for (int g = 0; g < 2; ++g) {
       tc::mbar_init(s_full(g), 1u);
       tc::mbar_init(p_full(g), 32u * kGroupWarps);
@@ -233,41 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     tc::fence_mbar_init();
   }
   const int page0 = tile0 * (kBN / kPage);
-  {
-    const int np = min(n_tiles * (kBN / kPage), kMaxPages);
-    for (int i = tid; i < np; i += kThreads) s_pages[i] = q8::page_of(bt_row, page0 + i, p.max_blocks, p.num_pages);
-  }
-  // ---- Q tiles -> shared memory as fp16, swizzled K-major; D / 8 neighbouring lanes share a row ----
-  {
-    constexpr int CPR = D / 8;
-    const int rows = ALT ? kBM : 2 * kBM;
-    for (int e = tid; e < rows * CPR; e += kThreads) {  // kThreads and rows * CPR are multiples of 32
-      const int m = e / CPR, ch = e % CPR, r = rt.row0 + m;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (r < rt.n_rows)
-        raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) +
-                                                   static_cast<int64_t>(rt.q0 + r / p.n_rep) * p.q_st +
-                                                   static_cast<int64_t>(hkv * p.n_rep + r % p.n_rep) * p.q_sh) + ch);
-      const T* x = reinterpret_cast<const T*>(&raw);
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(Elem<T>::to_f(x[i])) & 0x7fffffffu);
-#pragma unroll
-      for (int o = 1; o < CPR; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      // rows of zeros, or not finite, stay as they are
-      int qe = static_cast<int>(amax >> 23) - 127 - 14;
-      qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
-      uint32_t y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = pack2<__half>(Elem<T>::to_f(x[2 * i]) * inv, Elem<T>::to_f(x[2 * i + 1]) * inv);
-      sts128(qs + (m / kBM) * L::kQ + (ch >> 3) * (kBM * 128) + sw_off(m % kBM, ch & 7), y[0], y[1], y[2], y[3]);
-      if (ch == 0) s_qf[m] = __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
-    }
-    tc::fence_proxy_async_smem();
-  }
   tc::tc_fence_before();
-  __syncthreads();  // barriers initialised, TMEM address published, pages and Q staged
+  __syncthreads();  // barriers initialised, TMEM address published; from here on every role goes its own way
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   auto t_s = [&](int g) { return tmem + static_cast<uint32_t>(g * 256); };
@@ -282,11 +255,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   if (warp >= kConvWarp && warp < kMmaWarp) {
     // =================== converters ===================
     regs_dec<kRegsConv>();
+    const int ct = tid - kConvWarp * 32;
+    {
+      const int np = min(n_tiles * (kBN / kPage), kMaxPages);
+      for (int i = ct; i < np; i += 32 * kConvWarps) s_pages[i] = q8::page_of(bt_row, page0 + i, p.max_blocks, p.num_pages);
+      asm volatile("bar.sync 1, %0;\n" ::"n"(32 * (kConvWarps + 1)) : "memory");  // with the scale warp
+    }
     // Thread ct handles 16-code piece ct % 4 of each 64-code block of rows ct / 4 + RS i: a quarter warp then
     // stores whole swizzled rows of one block, without bank conflicts.
     constexpr int RS = 8 * kConvWarps, N = kBN / RS, DB = L::kDB;
     constexpr uint32_t kSlot = 32 * kConvWarps * 16;  // staging bytes of one piece of every thread
-    const int ct = tid - kConvWarp * 32;
     const int ch = ct & 3, r0 = ct >> 2;
     const int64_t in_page = static_cast<int64_t>(r0 & 15) * p.Hkv * D + static_cast<int64_t>(hkv) * D + ch * 16;
     const uint8_t *kp = p.kc + in_page, *vp = p.vc + in_page;
@@ -422,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       }
     };
     if (warp == kScaleWarp) {
+      asm volatile("bar.sync 1, %0;\n" ::"n"(32 * (kConvWarps + 1)) : "memory");  // s_pages is there
       auto fetch_scales = [&](const uint8_t* scales, int t) -> uint32_t {  // bytes of tokens 4 lane .. 4 lane + 3
         const int page = lane * 4 < rt.kv_end - (tile0 + t) * kBN ? page_at(t * (kBN / kPage) + lane / 4) : -1;
         return page < 0 ? 0u : __ldg(reinterpret_cast<const uint32_t*>(scales + page * p.scale_stride + hkv * kPage) + lane % 4);
@@ -479,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
         if (t + 2 < n_tiles) ksc_next = fetch_scales(p.ks, t + 2), vsc_next = fetch_scales(p.vs, t + 2);
       }
     }
-    bool ok = warp == kMmaWarp;
+    bool ok = warp == kMmaWarp && tc::mbar_wait(q_full, 0);
     for (int g = 0; ok && g < 2; ++g) {
       const int t = tile_at(g, 0);
       if (t >= n_tiles) break;
@@ -521,7 +500,42 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     const uint32_t ts = t_s(g) + lane_base + sc0, to = t_o(g) + lane_base + oc0;
     const uint32_t bar_id = 2 + g * 4 + rq;  // the two warps that share these rows
     float* mxg = s_mx + g * 4 * kBM;
-    const float qf = s_qf[(ALT ? 0 : g * kBM) + row];
+    // ---- Q tiles -> shared memory as fp16, swizzled K-major; D / 8 neighbouring lanes share a row ----
+    {
+      constexpr int CPR = D / 8, kPieces = L::kQTiles * kBM * CPR / (32 * 2 * kGroupWarps);  // per thread
+      uint4 raw[kPieces];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int e = tid + i * (32 * 2 * kGroupWarps), ch = e % CPR, qr = rt.row0 + e / CPR;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (qr < rt.n_rows)
+          raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) +
+                                                        static_cast<int64_t>(rt.q0 + qr / p.n_rep) * p.q_st +
+                                                        static_cast<int64_t>(hkv * p.n_rep + qr % p.n_rep) * p.q_sh) + ch);
+      }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int e = tid + i * (32 * 2 * kGroupWarps), m = e / CPR, ch = e % CPR;
+        const T* x = reinterpret_cast<const T*>(&raw[i]);
+        uint32_t amax = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) amax = max(amax, __float_as_uint(Elem<T>::to_f(x[u])) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < CPR; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        // rows of zeros, or not finite, stay as they are
+        int qe = static_cast<int>(amax >> 23) - 127 - 14;
+        qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
+        const float inv = __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
+        uint32_t y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] = pack2<__half>(Elem<T>::to_f(x[2 * u]) * inv, Elem<T>::to_f(x[2 * u + 1]) * inv);
+        sts128(qs + (m / kBM) * L::kQ + (ch >> 3) * (kBM * 128) + sw_off(m % kBM, ch & 7), y[0], y[1], y[2], y[3]);
+        if (ch == 0) s_qf[m] = __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
+      }
+      tc::fence_proxy_async_smem();
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(q_full) : "memory");
+    }
+    float qf = 1.f;  // this row's q factor: there once the first S is
     float m_ref = -INFINITY, l_run = 0.f;
     int vref = -1;  // reference of the values in O
     bool failed = false, row_nan = false;
@@ -535,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       const int t = tile_at(g, k);
       wait(s_full(g), k & 1);
       tc::tc_fence_after();
+      if (k == 0) qf = s_qf[(ALT ? 0 : g * kBM) + row];
       const TileInfo& info = s_info[t % kInfo];
       const float scale = info.scale * qf;
       const int tbase = t * kBN + sc0;
@@ -660,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     // l holds 2^kWOff times the sum; O the same times 2^-(vref - 127)
     const float inv = none ? 0.f : (bad || !all_ok) ? nan : 1.f / l_row;
     const float lse = !all_ok ? nan : none ? -INFINITY : (m_ref - kWOff + log2f(l_row)) * kLn2;
-    const int vexp = vref - 127;
+    const float vf = vref < 0 ? 0.f : q8::scale_of(vref);
     const int64_t o = static_cast<int64_t>(rt.q0 + tok) * p.Hq + hkv * p.n_rep + (valid ? r % p.n_rep : 0);
     const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
     const int part = ALT ? 2 * split + g : split;
@@ -677,20 +692,25 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       if (valid) {
         if (p.parts == 1) {
           T* dst = static_cast<T*>(p.out) + o * D + oc0 + c0;
+          uint32_t y[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            float v[8];
+          for (int c = 0; c < 32; c += 2) {
+            const bool blank = none && all_ok;
+            y[c >> 1] = pack2<T>(blank ? p.empty : acc[c] * inv * vf, blank ? p.empty : acc[c + 1] * inv * vf);
+          }
+          if ((reinterpret_cast<uintptr_t>(p.out) & 31) == 0) {
+            stg256(dst, y);
+            stg256(dst + 16, y + 8);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = none && all_ok ? 0.f : scalbnf(acc[c + i] * inv, vexp);
-            *reinterpret_cast<uint4*>(dst + c) =
-                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+            for (int c = 0; c < 16; c += 4) *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(y[c], y[c + 1], y[c + 2], y[c + 3]);
           }
         } else {
           float* dst = p.part_o + (part * all_rows + o) * D + oc0 + c0;
 #pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            *reinterpret_cast<float4*>(dst + c) = make_float4(scalbnf(acc[c] * inv, vexp), scalbnf(acc[c + 1] * inv, vexp),
-                                                              scalbnf(acc[c + 2] * inv, vexp), scalbnf(acc[c + 3] * inv, vexp));
+          for (int c = 0; c < 32; ++c) acc[c] = acc[c] * inv * vf;
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) stg256(dst + c, reinterpret_cast<const uint32_t*>(acc + c));
         }
       }
     }
@@ -715,33 +735,41 @@ __global__ void __launch_bounds__(256) chunk_q8_merge_kernel(const __grid_consta
   const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
   const int64_t o = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (o >= all_rows || q8::request_of(p.cu_q, p.B, static_cast<int>(o / p.Hq)) < 0) return;
-  float M = -INFINITY;
+  if (o >= all_rows || (p.cu_q != nullptr && q8::request_of(p.cu_q, p.B, static_cast<int>(o / p.Hq)) < 0)) return;
+  // lane i holds the log-sum-exp, then the weight, of parts i, i + 32, ... (at most kMaxParts of them)
+  float w[kMaxParts / 32], M = -INFINITY;
   bool nan = false;
-  for (int i = lane; i < p.parts; i += 32) {
-    const float x = p.part_lse[i * all_rows + o];
-    nan |= x != x;
-    M = fmaxf(M, x);
+#pragma unroll
+  for (int u = 0; u < kMaxParts / 32; ++u) {
+    w[u] = u * 32 + lane < p.parts ? p.part_lse[(u * 32 + lane) * all_rows + o] : -INFINITY;
+    nan |= w[u] != w[u];
+    M = fmaxf(M, w[u]);
   }
   for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
   nan = __any_sync(0xffffffffu, nan);
   float a[C] = {}, W = 0.f;
-  if (M != -INFINITY) {
-#pragma unroll 4
-    for (int i = 0; i < p.parts; ++i) {
-      const float x = p.part_lse[i * all_rows + o];
-      if (x == -INFINITY) continue;
-      const float w = exp2f((x - M) * 1.4426950408889634f);
-      W += w;
-      const float* src = p.part_o + (i * all_rows + o) * D + lane * C;
 #pragma unroll
-      for (int k = 0; k < C; ++k) a[k] += w * src[k];
+  for (int u = 0; u < kMaxParts / 32; ++u) {
+    w[u] = w[u] == -INFINITY ? 0.f : exp2f((w[u] - M) * 1.4426950408889634f);
+    W += w[u];
+  }
+  for (int s = 16; s > 0; s >>= 1) W += __shfl_xor_sync(0xffffffffu, W, s);
+#pragma unroll
+  for (int u = 0; u < kMaxParts / 32; ++u) {
+    const int n = min(32, p.parts - u * 32);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w[u], i);
+      const float* src = p.part_o + ((u * 32 + i) * all_rows + o) * D + lane * C;  // a part without tokens holds zeros
+#pragma unroll
+      for (int k = 0; k < C; ++k) a[k] += wi * src[k];
     }
   }
-  const float inv = nan ? __int_as_float(0x7fc00000) : M == -INFINITY ? 0.f : 1.f / W;
+  const bool blank = M == -INFINITY && !nan;
+  const float inv = nan ? __int_as_float(0x7fc00000) : blank ? 0.f : 1.f / W;
   T* dst = static_cast<T*>(p.out) + o * D + lane * C;
 #pragma unroll
-  for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(a[k] * inv, a[k + 1] * inv);
+  for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(blank ? p.empty : a[k] * inv, blank ? p.empty : a[k + 1] * inv);
   if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = nan ? inv : M == -INFINITY ? -INFINITY : M + logf(W);
 }
 

@@ -226,7 +226,6 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   constexpr int CH = D / 16;              // 16-byte pieces per row
   constexpr int KS = D / 16;              // MMA k-steps of S
   constexpr int MT = D / 16;              // 16-row tiles of O^T
-  constexpr bool kEarlyV = NT <= 2;       // V codes into registers before the softmax, which hides their latency
 
   int* prefix = reinterpret_cast<int*>(smem + NW * NS * STAGEB);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -394,11 +393,9 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         const int tok = (lane & 7) + 8 * ((lane >> 3) & 1);
         ldmatrix_x4_trans(sv + piece<D>(tok, mt + (lane >> 4)), r[0], r[1], r[2], r[3]);
       };
-      uint32_t vr[kEarlyV ? MT / 2 : 1][4];
-      if constexpr (kEarlyV) {
+      uint32_t vr[MT / 2][4];  // into registers before the softmax, which hides their latency
 #pragma unroll
-        for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
-      }
+      for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
       const bool ok0 = g < live, ok1 = g + 8 < live;
       const int kb0 = lds_u8(ss + g), kb1 = lds_u8(ss + g + 8);
       int vb0 = ok0 ? lds_u8(ss + 16 + g) : 0, vb1 = ok1 ? lds_u8(ss + 16 + g + 8) : 0;
@@ -422,15 +419,13 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
             q8::e4m3x4_to_f16x4(wb[w], a[1], a[3]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816<__half>(NT <= 2 && (w & 1) ? s2[nt] : s[nt], a, qb[nt][4 * j + w][0], qb[nt][4 * j + w][1]);
+              mma16816<__half>(w & 1 ? s2[nt] : s[nt], a, qb[nt][4 * j + w][0], qb[nt][4 * j + w][1]);
           }
         }
-        if constexpr (NT <= 2) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
-        }
+          for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
       }
       // ---- scores, online softmax in log2 ----
       const float kf0 = q8::scale_of(kb0), kf1 = q8::scale_of(kb1);
@@ -494,10 +489,8 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
           if (vb0 == q8::kNanByte) vb0 = 0;
           if (vb1 == q8::kNanByte) vb1 = 0;
           __syncwarp();
-          if constexpr (kEarlyV) {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
-          }
+          for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
         }
         const int vmax = __reduce_max_sync(0xffffffffu, max(vb0, vb1));
         if (vmax > vref) {
@@ -543,9 +536,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       // ---- O^T += V^T P^T ----
 #pragma unroll
       for (int mt = 0; mt < MT; mt += 2) {
-        uint32_t late[4];
-        if constexpr (!kEarlyV) load_v(mt, late);
-        const uint32_t* r = kEarlyV ? vr[kEarlyV ? mt / 2 : 0] : late;
+        const uint32_t* r = vr[mt / 2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           // bytes (token 2c: d, d + 1; token 2c + 1: d, d + 1) -> (d: both tokens), (d + 1: both tokens)
@@ -578,6 +569,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         if (r >= it.n_rows) continue;
         const bool none = m[nt][e] == -INFINITY && L == 0.f;
         const float inv = none ? 0.f : 1.f / L;
+        const float vf = q8::scale_of(vref), vd = 1.f / (1 << kWOff);  // the weights' unit, in two exact steps
         const float lse = none ? -INFINITY : (m[nt][e] + log2f(L)) * kLn2;
         const int64_t o = static_cast<int64_t>(it.q0 + r / p.n_rep) * p.Hq + h * p.n_rep + r % p.n_rep;
         const int64_t po = (static_cast<int64_t>(slot) * p.Hkv + h) * R + rl;
@@ -585,8 +577,8 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
           T* dst = static_cast<T*>(p.out) + o * D + 2 * g;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            const float y0 = none ? p.empty : scalbnf(acc[nt][mt][e] * inv, vref - 127 - kWOff);
-            const float y1 = none ? p.empty : scalbnf(acc[nt][mt][2 + e] * inv, vref - 127 - kWOff);
+            const float y0 = none ? p.empty : acc[nt][mt][e] * inv * vd * vf;
+            const float y1 = none ? p.empty : acc[nt][mt][2 + e] * inv * vd * vf;
             *reinterpret_cast<uint32_t*>(dst + mt * 16) = pack2<T>(y0, y1);
           }
           if (g == 0 && p.lse_out != nullptr) p.lse_out[o] = lse;
@@ -595,8 +587,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
             *reinterpret_cast<float2*>(dst + mt * 16) =
-                make_float2(scalbnf(acc[nt][mt][e] * inv, vref - 127 - kWOff),
-                            scalbnf(acc[nt][mt][2 + e] * inv, vref - 127 - kWOff));
+                make_float2(acc[nt][mt][e] * inv * vd * vf, acc[nt][mt][2 + e] * inv * vd * vf);
           if (g == 0) p.part_lse[po] = lse;
         }
       }
@@ -708,30 +699,49 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 constexpr int kMaxSplitItems = 4096;  // items whose page counts fit beside the ring in shared memory
 
-// Rows per request and KV head above which the tensor-core chunk kernel takes over.
-constexpr int kTcRows = 32;
+// Rows per request and KV head above which the tensor-core chunk kernel takes over (head_dim 64 and 128,
+// positive softmax scale).  Measured, 16 requests of 8192 tokens, 8 KV heads, this kernel / that one: head_dim
+// 128 16 rows 116 / 166 us, 32 rows 222 / 166; head_dim 64 77 / 132, 222 / 133.
+constexpr int kTcRows = 16;
+
+// CTAs per row tile of the chunk kernel, each a share of its tokens.  Estimated in K/V tiles of 128
+// tokens: a CTA costs its tiles and about nine more (start, first tile, last output), and the CTAs run
+// in waves of one per SM.  Measured (32 heads, 8 KV heads, head_dim 128), 1 / chosen split: 512 new tokens of
+// 32768 732 / 395 us, 128 new of 32768 718 / 120; 2048 new of 32768 1461 (4 splits: 1449, the parts' traffic
+// eats the gain of a fuller last wave).  The host does not see the lengths of a batch, and with one CTA per row tile its longest
+// request sets the time: a batch that fits one wave is split in two at least (16 x 16 new over 2000-16000
+// tokens: 282 / 181 us; 16 x 32 over 8192 each 178 / 205).
+int choose_splits(int64_t ctas, int B, int64_t tokens, int most) {
+  const int64_t sms = sm_count();
+  const float tiles = static_cast<float>(tokens) / 128.f;
+  if (ctas >= 2 * sms) return 1;
+  most = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(most), (tokens + 511) / 512)));
+  int best = 1;
+  float least = 1e30f;
+  for (int s = B > 1 && ctas <= sms ? min(2, most) : 1; s <= most; ++s) {
+    const float t = static_cast<float>((ctas * s + sms - 1) / sms) * (tiles / s + 9.f);
+    if (t < least) least = t, best = s;
+  }
+  return best;
+}
 
 struct Plan {
   int tc, alt, splits, parts;  // chunk_q8_tc.cu's, else the rest
-  int nt, nw, ns, groups, hp, pl, grid, tiles, n_items, split;
+  int nt, nw, groups, hp, pl, grid, tiles, n_items, split;
   size_t lse_off, o_off, bytes;
 };
 
-// Rows per tile: the smallest of {8, 16, 512 * 8 / D} that holds a request's rows (a wider tile reads
-// K and V once for more rows; its accumulators are what the register file holds).
 Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max_blocks, float scale) {
   Plan pl{};
   const int64_t rows = static_cast<int64_t>(max_q) * n_rep;
-  if (D <= 128 && max_q > 1 && rows > kTcRows && scale > 0.f) {
+  if (D <= 128 && rows > kTcRows && scale > 0.f) {
     pl.tc = 1;
     pl.alt = rows <= 128;
     const int64_t tiles = (rows + (pl.alt ? 127 : 255)) / (pl.alt ? 128 : 256);
     const int64_t ctas = tiles * B * Hkv;
     pl.tiles = static_cast<int>(tiles);
     pl.n_items = tiles * B < (1LL << 30) && ctas < (1LL << 30) ? static_cast<int>(tiles * B) : -1;
-    // split the tokens where the row tiles alone leave SMs idle, down to 512 tokens a split
-    const int64_t fill = ctas > 0 ? sm_count() / ctas : 1, most = (static_cast<int64_t>(max_blocks) * kPage + 511) / 512;
-    pl.splits = static_cast<int>(max(static_cast<int64_t>(1), min(min(fill, most), static_cast<int64_t>(64))));
+    pl.splits = choose_splits(ctas, B, static_cast<int64_t>(max_blocks) * kPage, pl.alt ? kMaxParts / 2 : kMaxParts);
     pl.parts = pl.splits * (pl.alt ? 2 : 1);
     if (pl.parts > 1) {
       const size_t all_rows = static_cast<size_t>(total_q) * Hkv * n_rep;
@@ -740,11 +750,8 @@ Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max
     }
     return pl;
   }
-  const int nt_max = 512 / D;
-  pl.nt = rows <= 8 ? 1 : (rows <= 16 || nt_max == 2) ? 2 : nt_max;
-  pl.nw = pl.nt == 1 ? 16 : 8;
-  pl.ns = D == 256 ? (pl.nt == 1 ? 1 : 3) : D == 128 ? (pl.nt == 1 ? 3 : 5) : (pl.nt == 1 ? 5 : 8);
-  if (D == 256 && pl.nt == 1) pl.nw = 8, pl.ns = 3;
+  pl.nt = rows <= 8 ? 1 : 2;
+  pl.nw = pl.nt == 1 && D <= 128 ? 16 : 8;
   pl.groups = (Hkv + 7) / 8;
   pl.hp = (Hkv + pl.groups - 1) / pl.groups;
   pl.pl = pl.nw / pl.hp;
@@ -806,13 +813,11 @@ template <typename T>
 int dispatch(Q8Params& p, const Plan& pl, int D, cudaStream_t st) {
   if (D == 64) {
     if (pl.nt == 1) return launch_attend<T, 64, 1, 16, 5>(p, pl, st);
-    if (pl.nt == 2) return launch_attend<T, 64, 2, 8, 8>(p, pl, st);
-    return launch_attend<T, 64, 8, 8, 8>(p, pl, st);
+    return launch_attend<T, 64, 2, 8, 8>(p, pl, st);
   }
   if (D == 128) {
     if (pl.nt == 1) return launch_attend<T, 128, 1, 16, 3>(p, pl, st);
-    if (pl.nt == 2) return launch_attend<T, 128, 2, 8, 5>(p, pl, st);
-    return launch_attend<T, 128, 4, 8, 5>(p, pl, st);
+    return launch_attend<T, 128, 2, 8, 5>(p, pl, st);
   }
   if (pl.nt == 1) return launch_attend<T, 256, 1, 8, 3>(p, pl, st);
   return launch_attend<T, 256, 2, 8, 3>(p, pl, st);
@@ -887,6 +892,7 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
     c.splits = pl.splits;
     c.parts = pl.parts;
     c.alt = pl.alt;
+    c.ranked = pl.n_items <= kMaxRanked && static_cast<int64_t>(pl.n_items) * pl.splits * num_kv_heads > sm_count();
     c.causal = causal;
     c.max_blocks = max_blocks;
     c.num_pages = num_pages;
@@ -897,6 +903,7 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
     c.scale_stride = scale_stride;
     c.bt_sb = bt_stride_b;
     c.scale_log2 = softmax_scale * 1.4426950408889634f;
+    c.empty = empty_nan ? NAN : 0.f;
     return chunk_q8_tc_launch(c, head_dim, dtype, static_cast<cudaStream_t>(stream));
   }
   Q8Params p{};
