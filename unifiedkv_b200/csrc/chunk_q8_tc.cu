@@ -99,12 +99,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// 32 bytes to a 32-byte boundary: a whole sector, where two 16-byte stores would write it in halves.
-__device__ __forceinline__ void stg256(void* dst, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
@@ -699,8 +693,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
             y[c >> 1] = pack2<T>(blank ? p.empty : acc[c] * inv * vf, blank ? p.empty : acc[c + 1] * inv * vf);
           }
           if ((reinterpret_cast<uintptr_t>(p.out) & 31) == 0) {
-            stg256(dst, y);
-            stg256(dst + 16, y + 8);
+            q8::stg256(dst, y);
+            q8::stg256(dst + 16, y + 8);
           } else {
 #pragma unroll
             for (int c = 0; c < 16; c += 4) *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(y[c], y[c + 1], y[c + 2], y[c + 3]);
@@ -710,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[c] = acc[c] * inv * vf;
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) stg256(dst + c, reinterpret_cast<const uint32_t*>(acc + c));
+          for (int c = 0; c < 32; c += 8) q8::stg256(dst + c, reinterpret_cast<const uint32_t*>(acc + c));
         }
       }
     }

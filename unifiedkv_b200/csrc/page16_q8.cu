@@ -701,8 +701,8 @@ constexpr int kMaxSplitItems = 4096;  // items whose page counts fit beside the 
 
 // Rows per request and KV head above which the tensor-core chunk kernel takes over (head_dim 64 and 128,
 // positive softmax scale).  Measured, 16 requests of 8192 tokens, 8 KV heads, this kernel / that one: head_dim
-// 128 16 rows 116 / 166 us, 32 rows 222 / 166; head_dim 64 77 / 132, 222 / 133.
-constexpr int kTcRows = 16;
+// 128: 32 rows 141 / 192 us, 64 rows 250 / 196; head_dim 64: 108 / 149, 189 / 153.
+constexpr int kTcRows = 32;
 
 // CTAs per row tile of the chunk kernel, each a share of its tokens.  Estimated in K/V tiles of 128
 // tokens: a CTA costs its tiles and about nine more (start, first tile, last output), and the CTAs run

@@ -48,6 +48,13 @@ __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32
       : "r"(w));
 }
 
+// 32 bytes to a 32-byte boundary: a whole sector, where two 16-byte stores would write it in halves.
+__device__ __forceinline__ void stg256(void* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // Page of request row `bt_row`, logical index j; -1 where the table has no such
 // page of the pool (past the table's width, negative as of an offloaded page, or
 // past the pool's end): such a page is never read or written.
