@@ -713,6 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       else if (p.lse_out != nullptr) p.lse_out[o] = lse;
     }
   }
+  // the merge may be scheduled from here on; it waits for this grid itself
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 0) {

@@ -594,6 +594,8 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
     }
   }
   cp_async_wait<0>();
+  // the combine may be scheduled from here on; it waits for this grid itself
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // Merges the items that several workers share.  CTA = (unit, one query row); a unit is an
@@ -611,6 +613,9 @@ __global__ void __launch_bounds__(kCombMaxWarps * 32) q8_combine_kernel(Q8Params
   __shared__ float s_acc[kCombMaxWarps][D];
   constexpr int C = D / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  // what the caller gave is there already: this grid starts after the attention kernel has
+  Item it{};
+  if (by_item) it = item_of<R>(p, blockIdx.x);
   pdl_wait();
   const int total = p.g_prefix[p.n_items];
   if (total == 0) return;
@@ -623,13 +628,13 @@ __global__ void __launch_bounds__(kCombMaxWarps * 32) q8_combine_kernel(Q8Params
     // this boundary is the item's first one: worker blockIdx.x has its first page
     const int first0 = p.g_prefix[item];
     if (first0 >= s || sh.start(blockIdx.x) > first0) return;
+    it = item_of<R>(p, item);
   }
   const int first = p.g_prefix[item], last = p.g_prefix[item + 1];
   if (first == last) return;  // written by the attention kernel
   const int c_lo = sh.owner(first), n = sh.owner(last - 1) - c_lo + 1;
   if (n == 1) return;  // one worker had all of it
   const int h = blockIdx.y / p.rows_max, rl = blockIdx.y % p.rows_max;
-  const Item it = item_of<R>(p, item);
   const int r = it.row0 + rl;
   if (r >= it.n_rows) return;
   // The item is the last one of worker c_lo (slot 1, or slot 0 if that worker begins with it) and the
