@@ -432,7 +432,8 @@ BPKV_API int bpkv_q8_dequantize(const void* k_codes, const void* v_codes, const 
  * tokens t <= seqlens_k - n + i (all of them when causal is 0) that have a page.
  * A query that sees none gives zeros, or NaN with empty_nan, and lse -inf.
  * Chunks longer than max_seqlen_q are cut there.
- * workspace: bpkv_q8_attention_workspace_size() bytes (may be 0). */
+ * workspace: bpkv_q8_attention_workspace_size() bytes (may be 0), 32-byte aligned;
+ * it may be reused as soon as later work on the stream may run. */
 BPKV_API size_t bpkv_q8_attention_workspace_size(int batch, int total_q, int num_q_heads,
                       int num_kv_heads, int head_dim, int max_blocks, int max_seqlen_q,
                       float softmax_scale);

@@ -183,10 +183,47 @@ def test_library_checks_without_a_gpu():
                       (dict(max_blocks=1 << 27), "max_blocks")):
         assert attend(**kw) == _lib.BPKV_ERR_SHAPE and token in _lib.last_error(), (kw, _lib.last_error())
     assert attend() == _lib.BPKV_ERR_WORKSPACE and "workspace" in _lib.last_error()
+    b = (a + 31) // 32 * 32
+    assert attend(ws=b + 16, ws_bytes=1 << 30) == _lib.BPKV_ERR_SHAPE and "workspace_alignment" in _lib.last_error()
+    assert attend(hq=2050, h=1025) == _lib.BPKV_ERR_SHAPE and "kv_heads" in _lib.last_error()
     assert attend(batch=0, total=0) == 0
     need = L.bpkv_q8_attention_workspace_size
     assert need(1, 1, 3, 2, 64, 9, 1, 0.1) == 0 and need(1, 1, 4, 2, 96, 9, 1, 0.1) == 0
     assert need(4, 4, 32, 8, 128, 9, 1, 0.1) > 0
+
+
+def test_missing_library_fails_loudly():
+    """Without the library every operator raises and nothing is computed (a fresh interpreter: the real library
+    is loaded in this one)."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = r'''
+import torch
+from pathlib import Path
+import unifiedkv_b200._lib as L
+L.LIB_PATH = Path("/nonexistent/libbpkv.so")
+from unifiedkv_b200 import kv_quant
+c = torch.zeros(2, 16, 1, 64, dtype=torch.float8_e4m3fn)
+s = torch.zeros(2, 1, 16, dtype=torch.uint8)
+kv = kv_quant.QuantPagedKV(c, c, s, s)
+x, bt, n = torch.zeros(1, 1, 64), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+cu = torch.tensor([0, 1], dtype=torch.int32)
+calls = [lambda: kv_quant.quantize_append(kv, x, x, bt, n), lambda: kv_quant.dequantize_pages(kv, bt, cu, 1),
+         lambda: kv_quant.page16_decode_attention_q8(x.half(), kv, bt, n, softmax_scale=0.1, n_rep=1),
+         lambda: kv_quant.paged_chunk_prefill_q8(x.half(), kv, bt, [0], [1])]
+for fn in calls:
+    try:
+        fn()
+    except RuntimeError as exc:
+        assert str(exc).startswith("page16_native_unavailable"), str(exc)
+    else:
+        raise AssertionError("ran without the library")
+print("ok")
+'''
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-3000:]
 
 
 def test_pool_bookkeeping_and_layout():

@@ -543,6 +543,84 @@ def test_side_stream_and_graphs(cuda):
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing has to have run before: kernels are loaded and set up while the stream is being captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = r'''
+import torch
+from unifiedkv_b200.kv_quant import QuantPagedKVPool, dequantize_pages, page16_decode_attention_q8, paged_chunk_prefill_q8, quantize_append
+dev = torch.device("cuda:0")
+pool = QuantPagedKVPool(16, 1, 2, 128, device=dev, n_total=30)
+kv = pool.layer(0)
+bt = torch.arange(30, dtype=torch.int32, device=dev).view(1, 30)
+n, cu = torch.tensor([200], dtype=torch.int32, device=dev), torch.tensor([0, 200], dtype=torch.int32, device=dev)
+q, k = torch.randn(200, 4, 128, device=dev).bfloat16(), torch.randn(200, 2, 128, device=dev).bfloat16()
+torch.cuda.synchronize()
+
+def step():
+    quantize_append(kv, k, k, bt, n, cu_seqlens_q=cu)
+    a = paged_chunk_prefill_q8(q, kv, bt, n_rep=2, cu_seqlens_q=cu, seqlens_k=n, max_seqlen_q=200)
+    b = paged_chunk_prefill_q8(q[:5], kv, bt, n_rep=2, cu_seqlens_q=cu.clamp(max=5), seqlens_k=n, max_seqlen_q=5)
+    return a, b, page16_decode_attention_q8(q[:1], kv, bt, n, softmax_scale=0.1, n_rep=2), *dequantize_pages(kv, bt, cu, 200)
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in out]
+assert all(torch.equal(x, y) for x, y in zip(got, step()))
+print("ok")
+'''
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-3000:]
+
+
+def test_sequence_bounds_past_the_rows_of_q(cuda):
+    """cu_seqlens that claim more rows than q has: the rows that are there are computed, none other is touched."""
+    for d, new in ((64, 5), (128, 60)):
+        kv = _fill(cuda, 12, 1, d, seed=60)
+        bt = _table(cuda, [100], 12, seed=61)
+        q = torch.randn(new, 2, d, device=cuda).bfloat16()
+        from unifiedkv_b200.kv_quant import paged_chunk_prefill_q8
+        whole = torch.cat([q, torch.zeros(20, 2, d, device=cuda, dtype=q.dtype)])
+        call = dict(softmax_scale=0.1, n_rep=2, cu_seqlens_q=_i32(cuda, [0, new + 20]), seqlens_k=_i32(cuda, [100]))
+        want = paged_chunk_prefill_q8(whole, kv, bt, max_seqlen_q=new + 20, **call)
+        got = paged_chunk_prefill_q8(q, kv, bt, max_seqlen_q=new + 20, **call)
+        torch.testing.assert_close(got.float(), want[:new].float(), rtol=2.0 ** -7, atol=2.0 ** -8)
+
+
+def test_tensors_of_another_device_are_refused(cuda):
+    from unifiedkv_b200.kv_quant import dequantize_pages, page16_decode_attention_q8, quantize_append
+    kv = _fill(cuda, 3, 2, 64, seed=62)
+    bt, n = torch.zeros(1, 2, dtype=torch.int32, device=cuda), _i32(cuda, [3])
+    x = torch.randn(1, 2, 64, device=cuda).bfloat16()
+    for call in (lambda: quantize_append(kv, x, x.cpu(), bt, n), lambda: quantize_append(kv, x, x, bt.cpu(), n),
+                 lambda: quantize_append(kv._replace(k_scales=kv.k_scales.cpu()), x, x, bt, n),
+                 lambda: dequantize_pages(kv, bt, torch.tensor([0, 2]), 2),
+                 lambda: page16_decode_attention_q8(x, kv, bt, n.cpu(), softmax_scale=0.1, n_rep=1)):
+        with pytest.raises(RuntimeError, match="shape_unsupported:device_cpu"):
+            call()
+
+
+@pytest.mark.parametrize("h_kv,n_rep,d", [(16, 2, 64), (33, 1, 128), (1, 32, 128)])
+def test_many_heads(cuda, h_kv, n_rep, d):
+    """More KV heads than a CTA's warps, one KV head for all: decode and chunks."""
+    from unifiedkv_b200.kv_quant import page16_decode_attention_q8
+    lens, new = [70, 300], [1, 1]
+    kv = _fill(cuda, 30, h_kv, d, seed=63)
+    bt = _table(cuda, lens, 30, seed=64)
+    q = torch.randn(2, h_kv * n_rep, d, device=cuda, generator=torch.Generator(device=cuda).manual_seed(10)).bfloat16()
+    out = page16_decode_attention_q8(q, kv, bt, _i32(cuda, lens), softmax_scale=d ** -0.5, n_rep=n_rep)
+    _check(out, None, q, kv, bt, lens, new, d ** -0.5)
+    q = torch.randn(43, h_kv * n_rep, d, device=cuda, generator=torch.Generator(device=cuda).manual_seed(11)).bfloat16()
+    out, lse = _chunk(cuda, q, kv, bt, lens, [3, 40], n_rep, d ** -0.5)
+    _check(out, lse, q, kv, bt, lens, [3, 40], d ** -0.5)
+
+
 def test_no_synchronisation_and_no_empty_launch(cuda):
     """Empty batches are answered without a launch; nothing waits for the device."""
     from unifiedkv_b200.kv_quant import dequantize_pages, paged_chunk_prefill_q8, quantize_append

@@ -23,10 +23,12 @@
 //    issues PV_A S_A' PV_B S_B' so that one group's softmax runs under the other's
 //    MMAs.  With more than 128 rows A and B are two row tiles over the same K/V tiles;
 //    with fewer (alternating) both hold the same rows and take every other K/V tile.
-//  * Softmax: online in exp2, a reference maximum moved only when it lags by 2^4, one
-//    in 8 exponentials on the FMA pipe.  Weights go to TMEM as fp16 in units of 2^-11 (off
-//    by 2^-11 of each, against 2^-8 for a bf16 output; nothing above 2^-35 of the row's
-//    largest vanishes); fp16 outputs take them as a high and a low part.
+//  * Softmax: online in exp2, a reference maximum moved only when it lags by 2^4.  Weights
+//    go to TMEM as fp16 in units of 2^-11 (off by 2^-11 of each, against 2^-8 for a bf16
+//    output; nothing above 2^-35 of the row's largest vanishes); fp16 outputs take them as
+//    a high and a low part.  (Exponentials on the FMA pipe, one in 4, 6 or 8: 1597, 1440,
+//    1439 us for 2048 new of 32768 tokens against 1440 with none: the special function
+//    unit is not what bounds the kernel.)
 //  * Few rows over long caches: the K/V tiles of an item are cut into splits, each a
 //    CTA; these (and the two groups when alternating) leave fp32 (o, lse) parts that
 //    chunk_q8_merge_kernel joins.
@@ -55,7 +57,6 @@ constexpr int kMaxPages = 1024;       // block-table entries staged in shared me
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescale = 4.f, kWOff = 11.f;  // weights <= 2^4, held times 2^11
 constexpr int kVHead = 6;                      // values are held as code * 2^(byte - vref), byte <= vref + 6
-constexpr int kEmuStride = 8;
 
 // What a K/V tile's scales come to, worked out once by the scale warp: for the converters a factor per row
 // (fp16 bits), for the softmax warps the rest.  A ring of 4; a slot is free again once P.V of its tile is done.
@@ -144,7 +145,7 @@ __device__ __forceinline__ RowTile row_tile(const ChunkQ8Params& p, int i) {
   r.row0 = (i % p.tiles) * rows;
   r.q0 = p.cu_q == nullptr ? r.b : __ldg(p.cu_q + r.b);
   r.n_q = p.cu_q == nullptr ? 1 : __ldg(p.cu_q + r.b + 1) - r.q0;
-  r.n_rows = r.n_q * p.n_rep;
+  r.n_rows = r.q0 < 0 ? 0 : min(r.n_q, p.total_q - r.q0) * p.n_rep;  // q has total_q rows, whatever cu_q says
   const int len = __ldg(p.lens + r.b);
   r.kv_end = 0;
   if (r.row0 < r.n_rows) {
@@ -609,17 +610,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           const uint64_t x2 = fma2(pk2(s[c], s[c + 1]), sc2, nm2);
-          uint64_t e2;
-          if ((c >> 1) % kEmuStride == kEmuStride - 1) {
-            e2 = exp2_poly2(x2);
-          } else {
-            float xa, xb;
-            up2(x2, xa, xb);
-            e2 = pk2(fast_exp2(xa), fast_exp2(xb));
-          }
-          sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], e2);
           float ea, eb;
-          up2(e2, ea, eb);
+          up2(x2, ea, eb);
+          ea = fast_exp2(ea), eb = fast_exp2(eb);
+          sum2[(c >> 1) & 1] = add2(sum2[(c >> 1) & 1], pk2(ea, eb));
           if constexpr (kTwoParts) {
             split2<__half>(ea, eb, hi[c >> 1], lo[c >> 1]);
           } else {

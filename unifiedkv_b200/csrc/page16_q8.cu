@@ -59,7 +59,7 @@ struct Q8Params {
   int32_t* g_prefix;    // workspace: [items + 1]
   float* part_lse;      // workspace: [2 W][Hkv][R]
   float* part_o;        // workspace: [2 W][Hkv][R][D]
-  int B, Hq, Hkv, n_rep, max_blocks, num_pages, tiles, n_items, split, causal, rows_max, hp, pl;
+  int B, total_q, Hq, Hkv, n_rep, max_blocks, num_pages, tiles, n_items, split, causal, rows_max, hp, pl;
   float empty;          // value of a row that sees no key
   int64_t q_st, q_sh, page_stride, scale_stride, bt_sb;
   float scale_log2;
@@ -82,7 +82,7 @@ __device__ __forceinline__ Item item_of(const Q8Params& p, int i) {
   it.row0 = (i % p.tiles) * R;
   it.q0 = p.cu_q == nullptr ? it.b : __ldg(p.cu_q + it.b);
   it.n_q = p.cu_q == nullptr ? 1 : __ldg(p.cu_q + it.b + 1) - it.q0;
-  it.n_rows = it.n_q * p.n_rep;
+  it.n_rows = it.q0 < 0 ? 0 : min(it.n_q, p.total_q - it.q0) * p.n_rep;  // q has total_q rows, whatever cu_q says
   it.len = __ldg(p.lens + it.b);
   return it;
 }
@@ -855,6 +855,7 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
   const char* what = "q8_attention_shape_unsupported";
   BPKV_CHECK_ARG(batch >= 0 && total_q >= 0 && num_q_heads > 0 && max_blocks >= 0 && num_pages >= 0, "%s:empty", what);
   BPKV_CHECK_ARG(num_kv_heads > 0 && num_q_heads % num_kv_heads == 0, "%s:gqa", what);
+  BPKV_CHECK_ARG(num_kv_heads <= 1024, "%s:kv_heads_%d", what, num_kv_heads);
   BPKV_CHECK_ARG(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s:head_dim_%d", what, head_dim);
   BPKV_CHECK_ARG(dtype == BPKV_F16 || dtype == BPKV_BF16, "%s:dtype_%d", what, dtype);
   BPKV_CHECK_ARG(cu_seqlens_q != nullptr || (max_seqlen_q == 1 && total_q == batch), "%s:max_seqlen_q", what);
@@ -875,6 +876,7 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
     set_error("q8_attention_workspace:need_%zu_bytes", pl.bytes);
     return BPKV_ERR_WORKSPACE;
   }
+  BPKV_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 31) == 0, "%s:workspace_alignment", what);
   if (pl.tc) {
     ChunkQ8Params c{};
     c.q = q;
@@ -927,6 +929,7 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
   p.part_lse = reinterpret_cast<float*>(ws + pl.lse_off);
   p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
   p.B = batch;
+  p.total_q = total_q;
   p.Hq = num_q_heads;
   p.Hkv = num_kv_heads;
   p.n_rep = n_rep;
