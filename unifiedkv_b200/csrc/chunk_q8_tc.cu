@@ -286,6 +286,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       sts128(b + sw_off(r0, 2 * ch), x[0], x[1], x[2], x[3]);
       sts128(b + sw_off(r0, 2 * ch + 1), x[4], x[5], x[6], x[7]);
     };
+    // this thread's pieces of half h and the factors of their rows, all asked for before any is used
+    auto take = [&](int h, const uint16_t* factors, uint4* c, uint32_t* f) {
+      cp_async_wait<(kDepth - 1) * N>();  // half h has come
+#pragma unroll
+      for (int i = 0; i < N * DB; ++i) c[i] = lds128(slot_of(h, i / DB) + (i % DB) * kSlot);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t x = factors[r0 + RS * i];
+        f[i] = x | x << 16;
+      }
+    };
     for (int h = 0; h < kDepth; ++h) {
 #pragma unroll
       for (int i = 0; i < N; ++i) fetch(h, i);
@@ -293,35 +304,29 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     bool ok = true;
     for (int t = 0; ok && t < n_tiles; ++t) {
       const TileInfo& info = s_info[t % kInfo];
-      auto factor = [&](const uint16_t* f, int i) {
-        const uint32_t x = f[r0 + RS * i];
-        return x | x << 16;
-      };
       ok = tc::mbar_wait(info_full(t), (t / kInfo) & 1);
       // ---- K ----
       if (ok && t >= kRing) ok = tc::mbar_wait(k_free(t), (t / kRing - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
       {
         const uint32_t dst = ks + (t % kRing) * L::kKV;
+        uint4 c[N * DB];
+        uint32_t f[N];
+        take(2 * t, info.kf, c, f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t f = factor(info.kf, i);
-          cp_async_wait<kDepth * N - 1>();  // the oldest row on its way has come
+        for (int i = 0; i < N * DB; ++i) {
+          const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+          uint32_t x[8];
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const uint4 c = lds128(slot_of(2 * t, i) + db * kSlot);
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-            uint32_t x[8];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              q8::e4m3x4_to_f16x4(w[u], x[2 * u], x[2 * u + 1]);  // NaN codes stay NaN
-              x[2 * u] = hmul2(x[2 * u], f);
-              x[2 * u + 1] = hmul2(x[2 * u + 1], f);
-            }
-            store(dst, i, db, x);
+          for (int u = 0; u < 4; ++u) {
+            q8::e4m3x4_to_f16x4(w[u], x[2 * u], x[2 * u + 1]);  // NaN codes stay NaN
+            x[2 * u] = hmul2(x[2 * u], f[i / DB]);
+            x[2 * u + 1] = hmul2(x[2 * u + 1], f[i / DB]);
           }
-          fetch(2 * t + kDepth, i);
+          store(dst, i / DB, i % DB, x);
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) fetch(2 * t + kDepth, i);
       }
       tc::fence_proxy_async_smem();
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(k_full(t)) : "memory");
@@ -330,27 +335,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       if (!__all_sync(0xffffffffu, ok)) break;
       {
         const uint32_t dst = vs + (t % kRing) * L::kKV;
+        uint4 c[N * DB];
+        uint32_t f[N];
+        take(2 * t + 1, info.vf, c, f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          uint32_t f = factor(info.vf, i);
-          const uint32_t keep = f == 0x7fff7fffu ? 0u : 0xffffffffu;  // a NaN row: its codes are taken out
-          f &= keep;
-          cp_async_wait<kDepth * N - 1>();
+        for (int i = 0; i < N * DB; ++i) {
+          const uint32_t keep = f[i / DB] == 0x7fff7fffu ? 0u : 0xffffffffu;  // a NaN row: its codes are taken out
+          const uint32_t w[4] = {c[i].x & keep, c[i].y & keep, c[i].z & keep, c[i].w & keep};
+          uint32_t x[8];
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const uint4 c = lds128(slot_of(2 * t + 1, i) + db * kSlot);
-            const uint32_t w[4] = {c.x & keep, c.y & keep, c.z & keep, c.w & keep};
-            uint32_t x[8];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              q8::e4m3x4_to_f16x4(w[u], x[2 * u], x[2 * u + 1]);
-              x[2 * u] = hmul2(x[2 * u], f);
-              x[2 * u + 1] = hmul2(x[2 * u + 1], f);
-            }
-            store(dst, i, db, x);
+          for (int u = 0; u < 4; ++u) {
+            q8::e4m3x4_to_f16x4(w[u], x[2 * u], x[2 * u + 1]);
+            x[2 * u] = hmul2(x[2 * u], f[i / DB] & keep);
+            x[2 * u + 1] = hmul2(x[2 * u + 1], f[i / DB] & keep);
           }
-          fetch(2 * t + 1 + kDepth, i);
+          store(dst, i / DB, i % DB, x);
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) fetch(2 * t + 1 + kDepth, i);
       }
       tc::fence_proxy_async_smem();
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(v_full(t)) : "memory");
