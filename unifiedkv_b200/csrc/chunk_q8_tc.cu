@@ -33,6 +33,12 @@
 //    CTA; these (and the two groups when alternating) leave fp32 (o, lse) parts that
 //    chunk_q8_merge_kernel joins.
 //  * Every wait is bounded (a poll count and 2 s); one that runs out ends in NaN rows.
+//
+// Measured (32 query heads, 8 KV heads, head_dim 128, bf16): 2048 new of 32768 tokens 1.45 ms, 732
+// TFLOP/s, 46 % of the measured cuBLAS burst (the 16-bit pages' kernel: 797); 8 x 512 over 900-16000
+// tokens 0.39 ms, 695.  With converters that store nothing 1.35 ms, with an eighth of the MMAs 1.17:
+// the softmax chain (S, maximum, weights, P.V, next S) of two groups bounds it, and the converters'
+// stores share the shared-memory port with the MMAs' operands.
 #include <type_traits>
 
 #include "chunk_q8.cuh"

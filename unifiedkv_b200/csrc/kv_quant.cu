@@ -3,12 +3,10 @@
 // Both are bound by HBM: a row is read once and written once, with a handful of
 // instructions per element.  A block takes a few tokens with all their heads: it looks
 // their slots up once (request, page, position), into shared memory, and its threads then
-// walk over the (token, head, piece) items, kUnroll at a time so that enough loads are in
-// flight.  head_dim / 16 neighbouring threads share a row, so a warp touches whole
-// 128-byte lines.  Measured at
-// 32768 tokens, 8 KV heads, head_dim 128, bf16 (201.9 MB): write 38 us, 81 % of the measured
-// copy rate (8 elements a thread, maxima in fp32: 50 us), read back 37.5 us, 82 % (stores of
-// half sectors: 43 us; more pieces a thread at once changed neither).
+// walk over the (token, head, 16-element piece) items.  head_dim / 16 neighbouring threads
+// share a row, so a warp touches whole 128-byte lines.  Measured at 32768 tokens, 8 KV heads,
+// head_dim 128, bf16 (201.9 MB): write 36 us, 86 % of the measured copy rate (8 elements a
+// thread, maxima in fp32: 50 us), read back 37.5 us, 82 % (stores of half sectors: 43 us).
 #include "q8.cuh"
 
 namespace bpkv {
@@ -178,11 +176,9 @@ __device__ __forceinline__ void values16(const uint4& c, float s, float* x) {
   }
 }
 
-constexpr int kReadUnroll = 2;
-
 template <typename T, int D>
 __global__ void __launch_bounds__(256) q8_read_kernel(ReadParams p) {
-  constexpr int G = D / 16, kUnroll = kReadUnroll;
+  constexpr int G = D / 16, kUnroll = 2;
   __shared__ Slots s;
   const int t0 = blockIdx.x * p.tokens, n_tok = min(p.tokens, p.total - t0);
   const int items = n_tok * p.Hkv * G;
@@ -233,10 +229,10 @@ __global__ void __launch_bounds__(256) q8_read_kernel(ReadParams p) {
   }
 }
 
-// Tokens of a block: enough items for every thread's unrolled loads, but no fewer blocks than the SMs can
-// hold twice over.
-int block_tokens(int total, int items_per_token, int unroll) {
-  const int fill = max(1, 256 * unroll / items_per_token);
+// Tokens of a block: two items a thread (one, four, eight: 38, 37, 42 us for the write that takes 36 with
+// two), but no fewer blocks than the SMs can hold twice over.
+int block_tokens(int total, int items_per_token) {
+  const int fill = max(1, 512 / items_per_token);
   return min(min(fill, kMaxTokens), max(1, total / (2 * sm_count())));
 }
 
@@ -279,7 +275,7 @@ extern "C" BPKV_API int bpkv_q8_append(const void* k_new, const void* v_new, voi
                  "q8_append_shape_unsupported:alignment");
   AppendParams p{k_new, v_new, static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), k_scales, v_scales,
                  block_table, cu_seqlens_q, seqlens_k, batch, total_q, num_kv_heads, max_blocks, num_pages,
-                 block_tokens(total_q, num_kv_heads * (head_dim / 16), 1), k_stride_t, k_stride_h, v_stride_t, v_stride_h, page_stride, scale_stride, bt_stride_b};
+                 block_tokens(total_q, num_kv_heads * (head_dim / 16)), k_stride_t, k_stride_h, v_stride_t, v_stride_h, page_stride, scale_stride, bt_stride_b};
   const unsigned grid = static_cast<unsigned>((total_q + p.tokens - 1) / p.tokens);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define BPKV_APPEND(T)                                                        \
@@ -318,7 +314,7 @@ extern "C" BPKV_API int bpkv_q8_dequantize(const void* k_codes, const void* v_co
                    out_stride_t % per32 == 0 && out_stride_h % per32 == 0;
   ReadParams p{static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scales, v_scales, block_table,
                cu_seqlens, starts, k_out, v_out, batch, total, num_kv_heads, max_blocks, num_pages,
-               block_tokens(total, num_kv_heads * (head_dim / 16), kReadUnroll), wide, page_stride,
+               block_tokens(total, num_kv_heads * (head_dim / 16)), wide, page_stride,
                scale_stride, bt_stride_b, out_stride_t, out_stride_h};
   const unsigned grid = static_cast<unsigned>((total + p.tokens - 1) / p.tokens);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
