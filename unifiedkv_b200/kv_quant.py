@@ -212,9 +212,10 @@ def _attention(what: str, q: torch.Tensor, kv: QuantPagedKV, block_table: torch.
                lse_out: Optional[torch.Tensor]) -> torch.Tensor:
     lib = _lib.lib()  # raises page16_native_unavailable when the library is missing
     n, h_kv, d = _check_kv(kv, what)
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise RuntimeError(f"{what}_shape_unsupported:q_dim_{q.dim()}")
-    total, h_q, dq = q.shape
+    total, h_q, dq = shape
     if dq != d:
         raise RuntimeError(f"{what}_shape_unsupported:head_dim_{dq}")
     if h_q == 0 or h_kv == 0 or h_q != h_kv * int(n_rep):
@@ -235,13 +236,14 @@ def _attention(what: str, q: torch.Tensor, kv: QuantPagedKV, block_table: torch.
         with torch.cuda.device(dev):
             return _attention(what, q, kv, bt, lens, cu, max_q, softmax_scale, n_rep, causal, lse_out)
     q = _aligned(q)
-    out = torch.empty((total, h_q, d), dtype=q.dtype, device=dev)
-    ws_bytes = lib.bpkv_q8_attention_workspace_size(B, total, h_q, h_kv, d, bt.shape[1], max_q, softmax_scale)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    out = q.new_empty(shape)
+    max_blocks = bt.shape[1]
+    ws_bytes = lib.bpkv_q8_attention_workspace_size(B, total, h_q, h_kv, d, max_blocks, max_q, softmax_scale)
+    ws = q.new_empty(ws_bytes // 2) if ws_bytes else None
     qs = q.stride()
     rc = lib.bpkv_q8_attention(
         q.data_ptr(), kv.k_codes.data_ptr(), kv.v_codes.data_ptr(), kv.k_scales.data_ptr(), kv.v_scales.data_ptr(),
-        bt.data_ptr(), _lib.ptr(cu), lens.data_ptr(), out.data_ptr(), _lib.ptr(lse_out), B, total, h_q, h_kv, d, bt.shape[1],
+        bt.data_ptr(), _lib.ptr(cu), lens.data_ptr(), out.data_ptr(), _lib.ptr(lse_out), B, total, h_q, h_kv, d, max_blocks,
         n, max_q, qs[0], qs[1], kv.k_codes.stride(0), kv.k_scales.stride(0), bt.stride(0), float(softmax_scale),
         int(causal), int(cu is None), code, _lib.ptr(ws), ws_bytes, _stream(dev.index))
     if rc:
