@@ -224,17 +224,20 @@ __device__ __forceinline__ uint32_t piece(int r, int ch) {
   return static_cast<uint32_t>(r * D + ((ch ^ x) << 4));
 }
 
-template <typename T, int D, int NT, int NW, int NS>
+// D: head_dim; DS: warps that share a KV head, DW dimensions each (2 for head_dim 256, whose accumulators would
+// take a warp's registers twice over).  They add their halves of every score through shared memory.
+template <typename T, int D, int DS, int NT, int NW, int NS>
 __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int R = 8 * NT;
-  constexpr int TILEB = 16 * D;
+  constexpr int R = 8 * NT, DW = D / DS;
+  constexpr int TILEB = 16 * DW;
   constexpr int STAGEB = 2 * TILEB + 64;  // K, V, 16 + 16 scale bytes, number of live rows
-  constexpr int CH = D / 16;              // 16-byte pieces per row
-  constexpr int KS = D / 16;              // MMA k-steps of S
-  constexpr int MT = D / 16;              // 16-row tiles of O^T
+  constexpr int CH = DW / 16;             // 16-byte pieces per row
+  constexpr int KS = DW / 16;             // MMA k-steps of S
+  constexpr int MT = DW / 16;             // 16-row tiles of O^T
 
-  int* prefix = reinterpret_cast<int*>(smem + NW * NS * STAGEB);
+  float4* s_pair = reinterpret_cast<float4*>(smem + NW * NS * STAGEB);  // DS == 2: [2 buffers][NW][NT][32]
+  int* prefix = reinterpret_cast<int*>(s_pair + (DS == 2 ? 2 * NW * NT * 32 : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int W = gridDim.x * p.pl;
   if (p.split) {
@@ -255,9 +258,13 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       if (d == 0 && p.lse_out != nullptr) p.lse_out[o] = -INFINITY;
     }
   }
-  const int h = blockIdx.y * p.hp + warp % p.hp;
-  const int worker = blockIdx.x * p.pl + warp / p.hp;
-  if (warp / p.hp >= p.pl || h >= p.Hkv) return;
+  const int part = warp % DS, hw = warp / DS;
+  const int h = blockIdx.y * p.hp + hw % p.hp;
+  const int worker = blockIdx.x * p.pl + hw / p.hp;
+  if (hw / p.hp >= p.pl || h >= p.Hkv) return;
+  // the two warps of a head meet here (DS == 2); they walk over the same pages
+  auto meet = [&]() { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + hw) : "memory"); };
+  int turn = 0;  // buffer of s_pair
   int s_beg = 0, s_end = 0;
   if (p.split) {
     const Shares sh(prefix[p.n_items], W);
@@ -271,7 +278,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   const int64_t row_stride = static_cast<int64_t>(p.Hkv) * D;
   // this lane's pieces are ch0 of rows tok0, tok0 + 32 / CH, ...
   const int tok0 = lane / CH, ch0 = lane % CH;
-  const int64_t lane_off = static_cast<int64_t>(h) * D + tok0 * row_stride + ch0 * 16;
+  const int64_t lane_off = static_cast<int64_t>(h) * D + part * DW + tok0 * row_stride + ch0 * 16;
   auto issue = [&](const Walk<R>& w, int stage) {
     const int page = w.page_id;
     // rows past the item's last visible token are zero-filled, so that what a page holds there never
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       const int tok = tok0 + r * (32 / CH);
       const bool ok = tok < live;
       const int64_t o = ok ? r * (32 / CH) * row_stride : 0;
-      const uint32_t so = piece<D>(tok, ch0);
+      const uint32_t so = piece<DW>(tok, ch0);
       cp_async16(sk + so, kp + o, ok);
       cp_async16(sk + TILEB + so, vp + o, ok);
     }
@@ -339,21 +346,28 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       const int r = it.row0 + 8 * nt + g;
       const bool ok = r < it.n_rows;
       const T* qr = static_cast<const T*>(p.q) + static_cast<int64_t>(it.q0 + (ok ? r / p.n_rep : 0)) * p.q_st +
-                    static_cast<int64_t>(h * p.n_rep + (ok ? r % p.n_rep : 0)) * p.q_sh;
+                    static_cast<int64_t>(h * p.n_rep + (ok ? r % p.n_rep : 0)) * p.q_sh + part * DW;
       uint4 raw[2 * (CH / 4)];
       uint32_t amax = 0;
 #pragma unroll
       for (int j = 0; j < CH / 4; ++j) {
-        const int ch = D == 64 ? c : 2 * c + (j & 1) + 8 * (j >> 1);
+        const int ch = DW == 64 ? c : 2 * c + (j & 1) + 8 * (j >> 1);
         const uint4* src = reinterpret_cast<const uint4*>(qr + ch * 16);
         raw[2 * j] = ok ? __ldg(src) : make_uint4(0, 0, 0, 0);
         raw[2 * j + 1] = ok ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
       }
       const T* e = reinterpret_cast<const T*>(raw);
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) amax = max(amax, __float_as_uint(Elem<T>::to_f(e[i])) & 0x7fffffffu);
+      for (int i = 0; i < DW / 4; ++i) amax = max(amax, __float_as_uint(Elem<T>::to_f(e[i])) & 0x7fffffffu);
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      if constexpr (DS == 2) {  // one exponent for the whole row
+        uint32_t* x = reinterpret_cast<uint32_t*>(s_pair + turn * NW * NT * 32);
+        x[warp * 32 + lane] = amax;
+        meet();
+        amax = max(amax, x[(warp ^ 1) * 32 + lane]);
+        turn ^= 1;
+      }
       // exponent that brings the largest element into [2^14, 2^15); rows of zeros, or not finite, stay as they are
       int qe = static_cast<int>(amax >> 23) - 127 - 14;
       qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
@@ -398,7 +412,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       // V codes: lane (mi, row) of ldmatrix addresses token (row + 8 (mi & 1)), piece mt + (mi >> 1)
       auto load_v = [&](int mt, uint32_t* r) {
         const int tok = (lane & 7) + 8 * ((lane >> 3) & 1);
-        ldmatrix_x4_trans(sv + piece<D>(tok, mt + (lane >> 4)), r[0], r[1], r[2], r[3]);
+        ldmatrix_x4_trans(sv + piece<DW>(tok, mt + (lane >> 4)), r[0], r[1], r[2], r[3]);
       };
       uint32_t vr[MT / 2][4];  // into registers before the softmax, which hides their latency
 #pragma unroll
@@ -416,8 +430,8 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
           for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
 #pragma unroll
         for (int j = 0; j < CH / 4; ++j) {
-          const int ch = D == 64 ? c : 2 * c + (j & 1) + 8 * (j >> 1);
-          const uint4 ka = lds128(sk + piece<D>(g, ch)), kb = lds128(sk + piece<D>(g + 8, ch));
+          const int ch = DW == 64 ? c : 2 * c + (j & 1) + 8 * (j >> 1);
+          const uint4 ka = lds128(sk + piece<DW>(g, ch)), kb = lds128(sk + piece<DW>(g + 8, ch));
           const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -433,6 +447,18 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
+        if constexpr (DS == 2) {
+          float4* x = s_pair + turn * NW * NT * 32;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) x[(warp * NT + nt) * 32 + lane] = make_float4(s[nt][0], s[nt][1], s[nt][2], s[nt][3]);
+          meet();
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float4 y = x[((warp ^ 1) * NT + nt) * 32 + lane];  // the sum of two has no order
+            s[nt][0] += y.x, s[nt][1] += y.y, s[nt][2] += y.z, s[nt][3] += y.w;
+          }
+          turn ^= 1;
+        }
       }
       // ---- scores, online softmax in log2 ----
       const float kf0 = q8::scale_of(kb0), kf1 = q8::scale_of(kb1);
@@ -491,7 +517,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
           for (int t = 0; t < kPage; ++t) {
             const bool bad = t < live && lds_u8(ss + 16 + t) == q8::kNanByte;
             if (bad && lane < CH)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(sv + piece<D>(t, lane)), "r"(0) : "memory");
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(sv + piece<DW>(t, lane)), "r"(0) : "memory");
           }
           if (vb0 == q8::kNanByte) vb0 = 0;
           if (vb1 == q8::kNanByte) vb1 = 0;
@@ -581,21 +607,21 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         const int64_t o = static_cast<int64_t>(it.q0 + r / p.n_rep) * p.Hq + h * p.n_rep + r % p.n_rep;
         const int64_t po = (static_cast<int64_t>(slot) * p.Hkv + h) * R + rl;
         if (whole) {
-          T* dst = static_cast<T*>(p.out) + o * D + 2 * g;
+          T* dst = static_cast<T*>(p.out) + o * D + part * DW + 2 * g;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             const float y0 = none ? p.empty : acc[nt][mt][e] * inv * vd * vf;
             const float y1 = none ? p.empty : acc[nt][mt][2 + e] * inv * vd * vf;
             *reinterpret_cast<uint32_t*>(dst + mt * 16) = pack2<T>(y0, y1);
           }
-          if (g == 0 && p.lse_out != nullptr) p.lse_out[o] = lse;
+          if (g == 0 && part == 0 && p.lse_out != nullptr) p.lse_out[o] = lse;
         } else {
-          float* dst = p.part_o + po * D + 2 * g;
+          float* dst = p.part_o + po * D + part * DW + 2 * g;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
             *reinterpret_cast<float2*>(dst + mt * 16) =
                 make_float2(acc[nt][mt][e] * inv * vd * vf, acc[nt][mt][2 + e] * inv * vd * vf);
-          if (g == 0) p.part_lse[po] = lse;
+          if (g == 0 && part == 0) p.part_lse[po] = lse;
         }
       }
     }
@@ -711,7 +737,8 @@ __global__ void __launch_bounds__(kCombMaxWarps * 32) q8_combine_kernel(Q8Params
 // ---- host side ----------------------------------------------------------------
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-constexpr int kMaxSplitItems = 4096;  // items whose page counts fit beside the ring in shared memory
+// Items whose page counts fit beside the rings in shared memory.
+constexpr int max_split_items(int D) { return D == 256 ? 2048 : 4096; }
 
 // Rows per request and KV head above which the tensor-core chunk kernel takes over (head_dim 64 and 128,
 // positive softmax scale).  Measured, 16 requests of 8192 tokens, 8 KV heads, this kernel / that one: head_dim
@@ -765,17 +792,18 @@ Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max
     return pl;
   }
   pl.nt = rows <= 8 ? 1 : 2;
-  pl.nw = pl.nt == 1 && D <= 128 ? 16 : 8;
-  pl.groups = (Hkv + 7) / 8;
+  pl.nw = pl.nt == 1 ? 16 : 8;
+  const int per_head = D == 256 ? 2 : 1, heads = min(8, pl.nw / per_head);  // warps of a head, heads of a CTA
+  pl.groups = (Hkv + heads - 1) / heads;
   pl.hp = (Hkv + pl.groups - 1) / pl.groups;
-  pl.pl = pl.nw / pl.hp;
+  pl.pl = pl.nw / per_head / pl.hp;
   const int sms = sm_count();
   pl.grid = max(1, min(sms / pl.groups, kMaxWorkers / pl.pl));
   const int64_t tiles = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
   const int64_t items = tiles * B;
   pl.tiles = static_cast<int>(tiles);
   pl.n_items = items < (1LL << 30) ? static_cast<int>(items) : -1;
-  pl.split = items <= kMaxSplitItems;
+  pl.split = items <= max_split_items(D);
   if (pl.split) {
     const size_t slots = 2 * static_cast<size_t>(pl.grid) * pl.pl * Hkv * 8 * pl.nt;
     pl.lse_off = up256(sizeof(int32_t) * (items + 1));
@@ -787,16 +815,17 @@ Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max
 
 template <typename T, int D, int NT, int NW, int NS>
 int launch_attend(Q8Params& p, const Plan& pl, cudaStream_t st) {
-  const size_t ring = static_cast<size_t>(NW) * NS * (2 * 16 * D + 64);
+  constexpr int DS = D == 256 ? 2 : 1;
+  constexpr size_t ring = static_cast<size_t>(NW) * NS * (2 * 16 * (D / DS) + 64) + (DS == 2 ? 2 * NW * NT * 512 : 0);
   const size_t smem = ring + (pl.split ? sizeof(int) * (pl.n_items + 1) : 0);
-  static_assert(static_cast<size_t>(NW) * NS * (2 * 16 * D + 64) + 4 * (kMaxSplitItems + 1) + 1024 <= 232448, "shared memory");
-  auto kern = q8_attend_kernel<T, D, NT, NW, NS>;
+  static_assert(ring + 4 * (max_split_items(D) + 1) + 1024 <= 232448, "shared memory");
+  auto kern = q8_attend_kernel<T, D, DS, NT, NW, NS>;
   static bool raised[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !raised[dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(ring + sizeof(int) * (kMaxSplitItems + 1))) != cudaSuccess) {
+                             static_cast<int>(ring + sizeof(int) * (max_split_items(D) + 1))) != cudaSuccess) {
       set_error("q8_attention_launch:smem_attr");
       return BPKV_ERR_CUDA;
     }
@@ -833,8 +862,8 @@ int dispatch(Q8Params& p, const Plan& pl, int D, cudaStream_t st) {
     if (pl.nt == 1) return launch_attend<T, 128, 1, 16, 3>(p, pl, st);
     return launch_attend<T, 128, 2, 8, 5>(p, pl, st);
   }
-  if (pl.nt == 1) return launch_attend<T, 256, 1, 8, 3>(p, pl, st);
-  return launch_attend<T, 256, 2, 8, 3>(p, pl, st);
+  if (pl.nt == 1) return launch_attend<T, 256, 1, 16, 3>(p, pl, st);
+  return launch_attend<T, 256, 2, 8, 5>(p, pl, st);
 }
 
 }  // namespace
