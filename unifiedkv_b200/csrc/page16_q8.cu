@@ -167,7 +167,7 @@ struct Shares {
 template <int R>
 struct Walk {
   int item, page, end, next;  // next: first flattened page not yet visited (split), or next item (not split)
-  int tokens, page_id;        // of the item; of its page `page` (loader only)
+  int tokens, ids, ids_next, k;  // loader only: tokens of the item; lane l's ids are pages page - k + l, and 32 on
   const int32_t* bt_row;
   __device__ __forceinline__ bool live() const { return item >= 0; }
 };
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   const int tok0 = lane / CH, ch0 = lane % CH;
   const int64_t lane_off = static_cast<int64_t>(h) * D + part * DW + tok0 * row_stride + ch0 * 16;
   auto issue = [&](const Walk<R>& w, int stage) {
-    const int page = w.page_id;
+    const int page = __shfl_sync(0xffffffffu, w.ids, w.k);
     // rows past the item's last visible token are zero-filled, so that what a page holds there never
     // reaches the MMAs
     const int live = page < 0 ? 0 : min(kPage, w.tokens - w.page * kPage);
@@ -308,22 +308,30 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
   ld.item = cs.item = -1;
   ld.page = cs.page = ld.end = cs.end = 0;
   ld.next = cs.next = p.split ? s_beg : worker;
+  // 32 block-table entries a load, the next 32 under way: one dependent load per item, not per page
+  auto ids_at = [&](int page) { return page + lane < ld.end ? q8::page_of(ld.bt_row, page + lane, p.max_blocks, p.num_pages) : -1; };
   auto load_seek = [&]() {  // the loader's next item
     walk_next<R>(p, prefix, worker, W, s_end, ld);
     if (ld.live()) {
       const Item it = item_of<R>(p, ld.item);
       ld.tokens = item_tokens<R>(p, it);
       ld.bt_row = p.bt + static_cast<int64_t>(it.b) * p.bt_sb;
-      ld.page_id = q8::page_of(ld.bt_row, ld.page, p.max_blocks, p.num_pages);
+      ld.ids = ids_at(ld.page);
+      ld.ids_next = ids_at(ld.page + 32);
+      ld.k = 0;
     }
   };
   load_seek();
   auto load_one = [&](int stage) {
     if (ld.live()) {
       issue(ld, stage);
-      // the next page's id is fetched now, to be there when its turn comes
-      if (++ld.page == ld.end) load_seek();
-      else ld.page_id = q8::page_of(ld.bt_row, ld.page, p.max_blocks, p.num_pages);
+      if (++ld.page == ld.end) {
+        load_seek();
+      } else if (++ld.k == 32) {
+        ld.ids = ld.ids_next;
+        ld.ids_next = ids_at(ld.page + 32);
+        ld.k = 0;
+      }
     }
     cp_async_commit();
   };
