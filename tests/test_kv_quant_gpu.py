@@ -738,3 +738,74 @@ def test_chunks_of_values_that_are_not_finite(cuda):
     keep[first:] = False
     keep[3, 1] = keep[4, 0] = False
     assert torch.equal(out[keep], clean[keep])
+
+
+# ---- row tiles cut into shares: one request by the host, a batch by the device ------
+def _heads(kv, heads):
+    from unifiedkv_b200.kv_quant import QuantPagedKV
+    return QuantPagedKV(kv.k_codes[:, :, heads], kv.v_codes[:, :, heads], kv.k_scales[:, heads], kv.v_scales[:, heads])
+
+
+def _shared_pages(device, lens, n_pages, seed):
+    """A block table that comes back to the same few pages: long requests over a small cache."""
+    rng = np.random.default_rng(seed)
+    return torch.from_numpy(rng.integers(0, n_pages, (len(lens), -(-max(lens) // 16)), dtype=np.int32)).to(device)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_one_request_with_row_tiles_whole_and_cut(cuda, dtype):
+    """150 row tiles and KV heads, a little over the SMs: one row tile of each head whole, the other cut."""
+    h_kv, new, n, d = 75, 300, 5000, 64
+    kv = _fill(cuda, 20, h_kv, d, seed=60)
+    bt = _shared_pages(cuda, [n], 20, seed=61)
+    q = torch.randn(new, h_kv, d, device=cuda, generator=torch.Generator(device=cuda).manual_seed(10)).to(DT[dtype])
+    out, lse = _chunk(cuda, q, kv, bt, [n], [new], 1, 0.125)
+    heads = [0, 37, 74]
+    _check(out[:, heads], lse[:, heads], q[:, heads], _heads(kv, heads), bt, [n], [new], 0.125)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h_kv,n_rep,new,lens", [
+    (2, 4, [12, 8, 12, 1, 10, 0, 9], [5000, 300, 4100, 1, 4, 700, 0]),  # up to 48 rows; requests and rows that see nothing
+    (2, 3, [150, 90, 64], [5000, 200, 4200]),                           # two row tiles a request, the second not always there
+    (40, 1, [60, 60, 33, 60], [4200, 4200, 700, 4200]),                 # more CTAs than SMs
+])
+def test_batches_cut_by_their_lengths(cuda, dtype, d, h_kv, n_rep, new, lens):
+    kv = _fill(cuda, 20, h_kv, d, seed=62)
+    bt = _shared_pages(cuda, lens, 20, seed=63)
+    g = torch.Generator(device=cuda).manual_seed(11)
+    q = torch.randn(sum(new), h_kv * n_rep, d, generator=g, device=cuda).to(DT[dtype])
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, n_rep, d ** -0.5)
+    again, _ = _chunk(cuda, q, kv, bt, lens, new, n_rep, d ** -0.5)
+    assert torch.equal(out, again)
+    heads = sorted({0, h_kv // 2, h_kv - 1})
+    rows = [h * n_rep + r for h in heads for r in range(n_rep)]
+    _check(out[:, rows], lse[:, rows], q[:, rows], _heads(kv, heads), bt, lens, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("n_rep,new", [(4, [12, 9, 12]), (8, [40, 3, 64])])
+def test_a_captured_batch_is_cut_by_the_lengths_of_its_replay(cuda, n_rep, new):
+    from unifiedkv_b200.kv_quant import paged_chunk_prefill_q8
+    width = [6000, 6000, 6000]
+    kv = _fill(cuda, 20, 2, 128, seed=64)
+    bt = _shared_pages(cuda, width, 20, seed=65)
+    q = torch.randn(sum(new), 2 * n_rep, 128, device=cuda).bfloat16()
+    sk, cu = _i32(cuda, width), _cu(cuda, new)
+
+    def step():
+        lse = torch.full(q.shape[:2], 9.0, device=cuda)
+        return paged_chunk_prefill_q8(q, kv, bt, softmax_scale=0.1, n_rep=n_rep, cu_seqlens_q=cu, seqlens_k=sk,
+                                      max_seqlen_q=max(new), lse_out=lse), lse
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for lens in ([6000, 40, 700], [12, 0, 5999], [64, 64, 64], [2500, 2500, 6000]):
+        sk.copy_(_i32(cuda, lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        out, lse = (t.clone() for t in captured)
+        want = step()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        _check(out, lse, q, kv, bt, lens, new, 0.1)

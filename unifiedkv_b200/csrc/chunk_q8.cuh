@@ -18,15 +18,21 @@ struct ChunkQ8Params {
   float* lse_out;
   float* part_o;    // [parts][total_q * Hq][D]
   float* part_lse;  // [parts][total_q * Hq]
-  int B, Hq, Hkv, n_rep, tiles, splits, parts, alt, ranked, causal, max_blocks, num_pages, total_q;
-  // ranked: the row tiles are taken longest first, each CTA working the order out (at most kMaxRanked of them)
+  // How the row tiles are cut into pieces, a CTA per piece and KV head, longest row tile first.  One request: its
+  // last `whole` row tiles whole, the others in `shares` shares of their tokens each.  A batch: planned on the
+  // device from the lengths: pieces[i] = (row tile or -1, share | shares << 16), n_shares its shares; or (pieces
+  // null) all whole, and, if `ranked`, each CTA works the order out.
+  int2* pieces;       // [n_pieces]
+  int32_t* n_shares;  // [B * tiles]
+  int whole, shares, n_pieces, ranked, max_shares, sms;
+  int B, Hq, Hkv, n_rep, tiles, alt, causal, max_blocks, num_pages, total_q;
   int64_t q_st, q_sh, page_stride, scale_stride, bt_sb;
   float scale_log2;
   float empty;  // value of a row that sees no token
 };
 
-constexpr int kMaxRanked = 512;
-constexpr int kMaxParts = 64;  // of a row; a multiple of 32
+constexpr int kMaxRanked = 512;  // row tiles that can be put in order
+constexpr int kMaxParts = 64;     // of a row; a multiple of 32
 // head_dim 64 or 128, softmax scale > 0.
 int chunk_q8_tc_launch(const ChunkQ8Params& p, int head_dim, int dtype, cudaStream_t st);
 

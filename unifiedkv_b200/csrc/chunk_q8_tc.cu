@@ -29,14 +29,15 @@
 //    a high and a low part.  (Exponentials on the FMA pipe, one in 4, 6 or 8: 1597, 1440,
 //    1439 us for 2048 new of 32768 tokens against 1440 with none: the special function
 //    unit is not what bounds the kernel.)
-//  * Few rows over long caches: the K/V tiles of an item are cut into splits, each a
-//    CTA; these (and the two groups when alternating) leave fp32 (o, lse) parts that
-//    chunk_q8_merge_kernel joins.
+//  * The K/V tiles of row tiles are cut into shares where that fills the SMs better, a CTA
+//    each: by the host for one request, by chunk_q8_plan_kernel for a batch, whose lengths
+//    only the device knows.  Shares (and the two groups when alternating) leave fp32 (o, lse)
+//    parts that chunk_q8_merge_kernel joins.
 //  * Every wait is bounded (a poll count and 2 s); one that runs out ends in NaN rows.
 //
-// Measured (32 query heads, 8 KV heads, head_dim 128, bf16): 2048 new of 32768 tokens 1.45 ms, 732
-// TFLOP/s, 46 % of the measured cuBLAS burst (the 16-bit pages' kernel: 797); 8 x 512 over 900-16000
-// tokens 0.39 ms, 695.  With converters that store nothing 1.35 ms, with an eighth of the MMAs 1.17:
+// Measured (32 query heads, 8 KV heads, head_dim 128, bf16): 2048 new of 32768 tokens 1.33 ms, 801
+// TFLOP/s, 50 % of the measured cuBLAS burst (the 16-bit pages' kernel: 797); 8 x 512 over 900-16000
+// tokens 0.39 ms, 695.  Before row tiles were cut (1.45 ms) converters that store nothing took 1.35, an eighth of the MMAs 1.17:
 // the softmax chain (S, maximum, weights, P.V, next S) of two groups bounds it, and the converters'
 // stores share the shared-memory port with the MMAs' operands.
 #include <type_traits>
@@ -161,6 +162,91 @@ __device__ __forceinline__ RowTile row_tile(const ChunkQ8Params& p, int i) {
   return r;
 }
 
+// The plan of a batch.  Candidates: the `whole` longest row tiles, none to two full waves of CTAs, stay whole; the
+// tokens of each of the others are cut into s shares, or into shares of an s-th of the longest of them.  A candidate's
+// time is the work over the SMs (as in page16_q8.cu, choose_shares), plus the idle end of the last wave, as long as the
+// smallest piece, which starts last, but no less than the longest piece.
+constexpr int kPlanThreads = 1024;
+template <bool ALT>
+__global__ void __launch_bounds__(kPlanThreads) chunk_q8_plan_kernel(const __grid_constant__ ChunkQ8Params p) {
+  __shared__ int s_len[kMaxRanked], s_item[kMaxRanked], s_sorted[kMaxRanked], s_shares[kMaxRanked];
+  __shared__ unsigned long long s_best[kPlanThreads / 32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = p.B * p.tiles;
+  if (tid < n) {
+    const RowTile rt = row_tile<ALT>(p, tid);
+    s_len[tid] = rt.row0 >= rt.n_rows ? -1 : (rt.kv_end + kBN - 1) / kBN;
+  }
+  __syncthreads();
+  if (tid < n) {
+    const int t = s_len[tid];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += (s_len[j] > t) || (s_len[j] == t && j < tid);
+    s_item[rank] = tid;
+    s_sorted[rank] = t;
+  }
+  __syncthreads();
+  // candidate c: shares of an s-th (0) or s shares (1); full waves whole; s - 1
+  const int m = p.max_shares;
+  auto whole_of = [&](int c) { return min(n, c / m % 3 * p.sms / p.Hkv); };
+  auto piece_of = [&](int c) {
+    const int whole = whole_of(c), s = c % m + 1;
+    return whole < n ? max(1, (s_sorted[whole] + s - 1) / s) : 1;
+  };
+  auto shares_of = [&](int j, int c, int whole, int piece) {
+    const int t = s_sorted[j];
+    return t < 0 ? 0 : j < whole ? 1 : c >= 3 * m ? c % m + 1 : max(1, (t + piece - 1) / piece);
+  };
+  unsigned long long best = ~0ull;
+  for (int c = warp; c < 6 * m; c += kPlanThreads / 32) {
+    const int whole = whole_of(c), piece = piece_of(c);
+    if (c > 0 && (c % m == 0 || (c / m % 3 > 0 && (whole == 0 || whole >= n)))) continue;
+    unsigned tiles = 0, count = 0, cut = 0;
+    float least = INFINITY, longest = 0.f;
+    for (int j = lane; j < n; j += 32) {
+      const int k = shares_of(j, c, whole, piece);
+      if (k == 0) break;
+      const float size = static_cast<float>(s_sorted[j]) / k + (k > 1 ? 11.f : 9.f);
+      tiles += s_sorted[j];
+      count += k;
+      if (k > 1) cut += k;
+      least = fminf(least, size);
+      longest = fmaxf(longest, size);
+    }
+    tiles = __reduce_add_sync(0xffffffffu, tiles);
+    count = __reduce_add_sync(0xffffffffu, count);
+    cut = __reduce_add_sync(0xffffffffu, cut);
+    least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));  // not negative
+    longest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(longest)));
+    if (c > 0 && (count == 0 || count > static_cast<unsigned>(p.n_pieces))) continue;  // 0, nothing cut, always fits
+    const float per_sm = static_cast<float>(p.Hkv) / p.sms, idle = ceilf(count * per_sm) - count * per_sm;
+    const float cost = fmaxf((tiles + 9.f * count + 2.f * cut) * per_sm + (idle > 0.f ? idle * least : 0.f), longest);
+    best = min(best, static_cast<unsigned long long>(__float_as_uint(cost)) << 32 | static_cast<unsigned>(c));
+  }
+  if (lane == 0) s_best[warp] = best;
+  __syncthreads();
+  for (int i = 0; i < kPlanThreads / 32; ++i) best = min(best, s_best[i]);
+  const int c = static_cast<int>(best & 0xffffffffu);
+  const int shares = tid < n ? shares_of(tid, c, whole_of(c), piece_of(c)) : 0;
+  if (tid < n) s_shares[tid] = shares;
+  __syncthreads();
+  // pieces in the order of their size
+  int first = 0, total = 0;
+  const int64_t t = tid < n ? s_sorted[tid] : 0;
+  for (int j = 0; j < n; ++j) {
+    const int k = s_shares[j];
+    const int64_t d = s_sorted[j] * static_cast<int64_t>(shares) - t * k;
+    if (d > 0 || (d == 0 && j < tid)) first += k;
+    total += k;
+  }
+  if (tid < n) {
+    const int item = s_item[tid];
+    p.n_shares[item] = shares;
+    for (int i = 0; i < shares; ++i) p.pieces[first + i] = make_int2(item, i | shares << 16);
+  }
+  for (int i = total + tid; i < p.n_pieces; i += kPlanThreads) p.pieces[i] = make_int2(-1, 0);
+}
+
 template <typename T, int D, bool ALT>
 __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_constant__ ChunkQ8Params p) {
   using L = Layout<D, ALT>;
@@ -180,13 +266,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
 
   constexpr bool kTwoParts = std::is_same<T, __half>::value;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // ---- work item: (row tile, split, KV head), row tiles with most K/V tiles first ----
-  const int n_items = p.B * p.tiles;
+  // ---- work item: (row tile, share of its tokens, KV head) ----
   const int hkv = static_cast<int>(blockIdx.x % p.Hkv);
-  const int split = static_cast<int>(blockIdx.x / p.Hkv) % p.splits;
-  int item = static_cast<int>(blockIdx.x / p.Hkv) / p.splits;
-  if (p.ranked) {
+  int item = static_cast<int>(blockIdx.x / p.Hkv), share = 0, shares = 1;
+  if (p.pieces != nullptr) {
+    pdl_wait();
+    const int2 piece = __ldcg(p.pieces + item);
+    item = piece.x;
+    share = piece.y & 0xffff;
+    shares = piece.y >> 16;
+    if (item < 0) return;  // uniform across the CTA
+  } else if (p.B == 1) {
+    const int i = item - p.whole;
+    item = p.tiles - 1 - (i < 0 ? item : p.whole + i / p.shares);
+    if (i >= 0) share = i % p.shares, shares = p.shares;
+  } else if (p.ranked) {
     __shared__ int s_item;
+    const int n_items = p.B * p.tiles;
     for (int i = tid; i < n_items; i += kThreads) s_pages[i] = row_tile<ALT>(p, i).kv_end;
     __syncthreads();
     for (int i = tid; i < n_items; i += kThreads) {
@@ -201,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   const RowTile rt = row_tile<ALT>(p, item);
   if (rt.row0 >= rt.n_rows) return;  // uniform across the CTA, before any barrier or TMEM use
   const int all_tiles = (rt.kv_end + kBN - 1) / kBN;
-  const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
-  const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits) - tile0;
+  const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * share / shares);
+  const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (share + 1) / shares) - tile0;
   const int32_t* bt_row = p.bt + static_cast<int64_t>(rt.b) * p.bt_sb;
 
   auto k_full = [&](int t) { return smem_u32(&bars[t % kRing]); };
@@ -674,7 +770,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     const float vf = vref < 0 ? 0.f : q8::scale_of(vref);
     const int64_t o = static_cast<int64_t>(rt.q0 + tok) * p.Hq + hkv * p.n_rep + (valid ? r % p.n_rep : 0);
     const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
-    const int part = ALT ? 2 * split + g : split;
+    const int part = ALT ? 2 * share + g : share;
+    const bool whole = !ALT && shares == 1;
     if (all_ok && k > 0) tc::tc_fence_after();
 #pragma unroll
     for (int c0 = 0; c0 < kOC; c0 += 32) {
@@ -686,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
         for (int i = 0; i < 32; ++i) acc[i] = 0.f;
       }
       if (valid) {
-        if (p.parts == 1) {
+        if (whole) {
           T* dst = static_cast<T*>(p.out) + o * D + oc0 + c0;
           uint32_t y[16];
 #pragma unroll
@@ -711,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       }
     }
     if (valid && half == 0) {
-      if (p.parts > 1) p.part_lse[part * all_rows + o] = lse;
+      if (!whole) p.part_lse[part * all_rows + o] = lse;
       else if (p.lse_out != nullptr) p.lse_out[o] = lse;
     }
   }
@@ -725,50 +822,70 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   }
 }
 
-// Joins the parts of every row; one warp per row, D / 32 columns a lane.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) chunk_q8_merge_kernel(const __grid_constant__ ChunkQ8Params p) {
+// Joins the parts of every row that has some; one warp per row, D / 32 columns a lane.  The lanes of a warp
+// first look up 32 of its rows, most of which may have been written by their CTA.
+constexpr int kMergeWarps = 8;
+template <typename T, int D, bool ALT>
+__global__ void __launch_bounds__(32 * kMergeWarps) chunk_q8_merge_kernel(const __grid_constant__ ChunkQ8Params p) {
   constexpr int C = D / 32;
   pdl_wait();
   const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
-  const int64_t o = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kMergeWarps;
   const int lane = threadIdx.x & 31;
-  if (o >= all_rows || (p.cu_q != nullptr && q8::request_of(p.cu_q, p.B, static_cast<int>(o / p.Hq)) < 0)) return;
-  // lane i holds the log-sum-exp, then the weight, of parts i, i + 32, ... (at most kMaxParts of them)
-  float w[kMaxParts / 32], M = -INFINITY;
-  bool nan = false;
+  auto parts_of = [&](int64_t o) {
+    if (o >= all_rows) return 0;
+    const int tok = static_cast<int>(o / p.Hq), b = p.cu_q == nullptr ? tok : q8::request_of(p.cu_q, p.B, tok);
+    if (b < 0) return 0;
+    const int r = (p.cu_q == nullptr ? 0 : tok - __ldg(p.cu_q + b)) * p.n_rep + static_cast<int>(o % p.Hq) % p.n_rep;
+    const int tile = r / (ALT ? kBM : 2 * kBM);
+    if (tile >= p.tiles) return 0;
+    const int shares = p.pieces != nullptr ? __ldcg(p.n_shares + b * p.tiles + tile)
+                       : p.B == 1 && tile < p.tiles - p.whole ? p.shares : 1;
+    return ALT ? 2 * shares : shares > 1 ? shares : 0;
+  };
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5); first < all_rows; first += 32 * step) {
+    const int my_parts = parts_of(first + lane * step);
+    for (uint32_t left = __ballot_sync(0xffffffffu, my_parts > 0); left != 0; left &= left - 1) {
+      const int src_lane = __ffs(left) - 1;
+      const int parts = __shfl_sync(0xffffffffu, my_parts, src_lane);
+      const int64_t o = first + src_lane * step;
+      // lane i holds the log-sum-exp, then the weight, of parts i, i + 32, ... (at most kMaxParts of them)
+      float w[kMaxParts / 32], M = -INFINITY;
+      bool nan = false;
 #pragma unroll
-  for (int u = 0; u < kMaxParts / 32; ++u) {
-    w[u] = u * 32 + lane < p.parts ? p.part_lse[(u * 32 + lane) * all_rows + o] : -INFINITY;
-    nan |= w[u] != w[u];
-    M = fmaxf(M, w[u]);
-  }
-  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-  nan = __any_sync(0xffffffffu, nan);
-  float a[C] = {}, W = 0.f;
+      for (int u = 0; u < kMaxParts / 32; ++u) {
+        w[u] = u * 32 + lane < parts ? p.part_lse[(u * 32 + lane) * all_rows + o] : -INFINITY;
+        nan |= w[u] != w[u];
+        M = fmaxf(M, w[u]);
+      }
+      for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+      nan = __any_sync(0xffffffffu, nan);
+      float a[C] = {}, W = 0.f;
 #pragma unroll
-  for (int u = 0; u < kMaxParts / 32; ++u) {
-    w[u] = w[u] == -INFINITY ? 0.f : exp2f((w[u] - M) * 1.4426950408889634f);
-    W += w[u];
-  }
-  for (int s = 16; s > 0; s >>= 1) W += __shfl_xor_sync(0xffffffffu, W, s);
+      for (int u = 0; u < kMaxParts / 32; ++u) {
+        w[u] = w[u] == -INFINITY ? 0.f : exp2f((w[u] - M) * 1.4426950408889634f);
+        W += w[u];
+      }
+      for (int s = 16; s > 0; s >>= 1) W += __shfl_xor_sync(0xffffffffu, W, s);
 #pragma unroll
-  for (int u = 0; u < kMaxParts / 32; ++u) {
-    const int n = min(32, p.parts - u * 32);
+      for (int u = 0; u < kMaxParts / 32; ++u) {
+        const int n = min(32, parts - u * 32);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w[u], i);
-      const float* src = p.part_o + ((u * 32 + i) * all_rows + o) * D + lane * C;  // a part without tokens holds zeros
+        for (int i = 0; i < n; ++i) {
+          const float wi = __shfl_sync(0xffffffffu, w[u], i);
+          const float* src = p.part_o + ((u * 32 + i) * all_rows + o) * D + lane * C;  // a part without tokens holds zeros
 #pragma unroll
-      for (int k = 0; k < C; ++k) a[k] += wi * src[k];
+          for (int k = 0; k < C; ++k) a[k] += wi * src[k];
+        }
+      }
+      const bool blank = M == -INFINITY && !nan;
+      const float inv = nan ? __int_as_float(0x7fc00000) : blank ? 0.f : 1.f / W;
+      T* dst = static_cast<T*>(p.out) + o * D + lane * C;
+#pragma unroll
+      for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(blank ? p.empty : a[k] * inv, blank ? p.empty : a[k + 1] * inv);
+      if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = nan ? inv : M == -INFINITY ? -INFINITY : M + logf(W);
     }
   }
-  const bool blank = M == -INFINITY && !nan;
-  const float inv = nan ? __int_as_float(0x7fc00000) : blank ? 0.f : 1.f / W;
-  T* dst = static_cast<T*>(p.out) + o * D + lane * C;
-#pragma unroll
-  for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(blank ? p.empty : a[k] * inv, blank ? p.empty : a[k + 1] * inv);
-  if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = nan ? inv : M == -INFINITY ? -INFINITY : M + logf(W);
 }
 
 template <typename T, int D, bool ALT>
@@ -785,23 +902,29 @@ int launch_chunk(const ChunkQ8Params& p, cudaStream_t st) {
     }
     if (dev >= 0 && dev < 64) raised[dev] = true;
   }
-  kern<<<static_cast<unsigned>(p.B * p.tiles * p.splits * p.Hkv), kThreads, kBytes, st>>>(p);
-  return BPKV_OK;
+  const dim3 grid(static_cast<unsigned>(p.n_pieces) * p.Hkv);
+  cudaError_t e = cudaSuccess;
+  if (p.pieces != nullptr) {
+    chunk_q8_plan_kernel<ALT><<<1, kPlanThreads, 0, st>>>(p);
+    e = launch_pdl(kern, grid, dim3(kThreads), kBytes, st, p);
+  } else {
+    kern<<<grid, kThreads, kBytes, st>>>(p);
+  }
+  if (e == cudaSuccess && (ALT || p.max_shares > 1)) {
+    const int64_t rows = static_cast<int64_t>(p.total_q) * p.Hq;
+    const int64_t blocks = (rows + kMergeWarps - 1) / kMergeWarps, most = 8 * p.sms;
+    e = launch_pdl(chunk_q8_merge_kernel<T, D, ALT>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(32 * kMergeWarps), 0, st, p);
+  }
+  if (e != cudaSuccess) {
+    set_error("q8_attention_launch:%s", cudaGetErrorString(e));
+    return BPKV_ERR_CUDA;
+  }
+  BPKV_RETURN_LAUNCH("q8_attention_launch");
 }
 
 template <typename T, int D>
 int launch(const ChunkQ8Params& p, cudaStream_t st) {
-  const int rc = p.alt ? launch_chunk<T, D, true>(p, st) : launch_chunk<T, D, false>(p, st);
-  if (rc != BPKV_OK) return rc;
-  if (p.parts > 1) {
-    const int64_t rows = static_cast<int64_t>(p.total_q) * p.Hq;
-    const cudaError_t e = launch_pdl(chunk_q8_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, p);
-    if (e != cudaSuccess) {
-      set_error("q8_attention_launch:%s", cudaGetErrorString(e));
-      return BPKV_ERR_CUDA;
-    }
-  }
-  BPKV_RETURN_LAUNCH("q8_attention_launch");
+  return p.alt ? launch_chunk<T, D, true>(p, st) : launch_chunk<T, D, false>(p, st);
 }
 
 }  // namespace

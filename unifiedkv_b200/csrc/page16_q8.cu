@@ -753,31 +753,47 @@ constexpr int max_split_items(int D) { return D == 256 ? 2048 : 4096; }
 // 128: 32 rows 141 / 192 us, 64 rows 250 / 196; head_dim 64: 108 / 149, 189 / 153.
 constexpr int kTcRows = 32;
 
-// CTAs per row tile of the chunk kernel, each a share of its tokens.  Estimated in K/V tiles of 128
-// tokens: a CTA costs its tiles and about nine more (start, first tile, last output), and the CTAs run
-// in waves of one per SM.  Measured (32 heads, 8 KV heads, head_dim 128), 1 / chosen split: 512 new tokens of
-// 32768 732 / 395 us, 128 new of 32768 718 / 120; 2048 new of 32768 1461 (4 splits: 1449, the parts' traffic
-// eats the gain of a fuller last wave).  The host does not see the lengths of a batch, and with one CTA per row tile its longest
-// request sets the time: a batch that fits one wave is split in two at least (16 x 16 new over 2000-16000
-// tokens: 282 / 181 us; 16 x 32 over 8192 each 178 / 205).
-int choose_splits(int64_t ctas, int B, int64_t tokens, int most) {
-  const int64_t sms = sm_count();
+// The chunk kernel may cut the tokens of a row tile into shares, a CTA each.  Estimated in K/V tiles of 128
+// tokens: a CTA costs its tiles and about nine more (start, first tile, last output), and two more where it leaves
+// a part to be joined.
+//
+// One request: the row tiles are about as long as the table is wide, so the host chooses.  Candidates are
+// zero to two full waves of CTAs whole, the rest in s shares.  Measured (32 heads, 8 KV heads, head_dim
+// 128), 1 share / chosen: 512 new tokens of 32768 732 / 389 us, 128 new of 32768 718 / 117, 2048 new of 32768
+// (256 CTAs; 144 whole, 112 in 4 shares) 1461 / 1326.
+void choose_shares(int row_tiles, int Hkv, int64_t tokens, int most, int& whole, int& shares) {
+  const int sms = sm_count();
   const float tiles = static_cast<float>(tokens) / 128.f;
-  if (ctas >= 2 * sms) return 1;
-  most = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(most), (tokens + 511) / 512)));
-  int best = 1;
   float least = 1e30f;
-  for (int s = B > 1 && ctas <= sms ? min(2, most) : 1; s <= most; ++s) {
-    const float t = static_cast<float>((ctas * s + sms - 1) / sms) * (tiles / s + 9.f);
-    if (t < least) least = t, best = s;
+  for (int w = 0; w < 3; ++w) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(row_tiles), static_cast<int64_t>(w) * sms / Hkv));
+    if (w > 0 && (n == 0 || n == row_tiles)) continue;
+    for (int s = w == 0 ? 1 : 2; s <= most; ++s) {
+      const float pieces = n + static_cast<float>(s) * (row_tiles - n), waves = pieces * Hkv / sms;
+      const float cut = tiles / s + (s > 1 ? 11.f : 9.f), first = n > 0 ? tiles + 9.f : cut;
+      const float t = fmaxf(first, (n * (tiles + 9.f) + s * (row_tiles - n) * cut) * Hkv / sms + (ceilf(waves) - waves) * cut);
+      if (t < least) least = t, whole = n, shares = s;
+    }
   }
-  return best;
+}
+
+// A batch: chunk_q8_plan_kernel, which knows the lengths, chooses, if the table is wide enough (it costs
+// about 6 us, and the CTAs left over a little).  Measured, whole / planned: 8 x 64 new over 2048 tokens each 62 / 58
+// us, over 100-3900 103 / 54, 4 x 64 over 200-8000 190 / 55, 16 x 16 over 2000-16000 282 / 174, 16 x 32 over 8192 each
+// 178 / 179.
+// Shares that a row tile may be cut into: this bounds the CTAs and the parts' memory (8 x 256 rows per SM).  A
+// share is 512 tokens at least.
+constexpr int kPlanTokens = 2048;
+int most_shares(int64_t ctas, int64_t tokens, int most) {
+  const int64_t sms = sm_count();
+  const int64_t s = ctas <= sms / 2 ? 2 * sms / ctas : ctas <= 2 * sms ? max(static_cast<int64_t>(4), 4 * sms / ctas) : 1;
+  return static_cast<int>(max(static_cast<int64_t>(1), min(min(s, static_cast<int64_t>(most)), (tokens + 511) / 512)));
 }
 
 struct Plan {
-  int tc, alt, splits, parts;  // chunk_q8_tc.cu's, else the rest
+  int tc, alt, planned, ranked, whole, max_shares, n_pieces;  // chunk_q8_tc.cu's, else the rest
   int nt, nw, groups, hp, pl, grid, tiles, n_items, split;
-  size_t lse_off, o_off, bytes;
+  size_t shares_off, lse_off, o_off, bytes;
 };
 
 Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max_blocks, float scale) {
@@ -790,12 +806,27 @@ Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max
     const int64_t ctas = tiles * B * Hkv;
     pl.tiles = static_cast<int>(tiles);
     pl.n_items = tiles * B < (1LL << 30) && ctas < (1LL << 30) ? static_cast<int>(tiles * B) : -1;
-    pl.splits = choose_splits(ctas, B, static_cast<int64_t>(max_blocks) * kPage, pl.alt ? kMaxParts / 2 : kMaxParts);
-    pl.parts = pl.splits * (pl.alt ? 2 : 1);
-    if (pl.parts > 1) {
+    const int sms = sm_count();
+    const int64_t tokens = static_cast<int64_t>(max_blocks) * kPage;
+    pl.n_pieces = pl.n_items;
+    pl.max_shares = most_shares(ctas, tokens, pl.alt ? kMaxParts / 2 : kMaxParts);
+    if (B == 1 && pl.n_items > 0) {
+      choose_shares(pl.n_items, Hkv, tokens, pl.max_shares, pl.whole, pl.max_shares);
+      pl.n_pieces = pl.whole + (pl.n_items - pl.whole) * pl.max_shares;
+    } else if (pl.n_items > 0 && pl.n_items <= kMaxRanked && pl.max_shares > 1 && tokens >= kPlanTokens) {
+      pl.planned = 1;
+      pl.n_pieces = min(pl.n_items * pl.max_shares, pl.n_items + 2 * sms / Hkv);
+      pl.shares_off = up256(sizeof(int2) * pl.n_pieces);
+      pl.bytes = pl.lse_off = pl.shares_off + up256(sizeof(int32_t) * pl.n_items);
+    } else {
+      pl.max_shares = 1;
+      pl.ranked = pl.n_items <= kMaxRanked && ctas > sms;
+    }
+    const int parts = pl.max_shares * (pl.alt ? 2 : 1);
+    if (parts > 1) {
       const size_t all_rows = static_cast<size_t>(total_q) * Hkv * n_rep;
-      pl.o_off = up256(sizeof(float) * pl.parts * all_rows);
-      pl.bytes = pl.o_off + sizeof(float) * pl.parts * all_rows * D;
+      pl.o_off = pl.lse_off + up256(sizeof(float) * parts * all_rows);
+      pl.bytes = pl.o_off + sizeof(float) * parts * all_rows * D;
     }
     return pl;
   }
@@ -935,17 +966,24 @@ extern "C" BPKV_API int bpkv_q8_attention(const void* q, const void* k_codes, co
     c.lens = seqlens_k;
     c.out = out;
     c.lse_out = lse_out;
-    c.part_lse = static_cast<float*>(workspace);
-    c.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.o_off);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (pl.planned) {
+      c.pieces = reinterpret_cast<int2*>(ws);
+      c.n_shares = reinterpret_cast<int32_t*>(ws + pl.shares_off);
+    }
+    c.part_lse = reinterpret_cast<float*>(ws + pl.lse_off);
+    c.part_o = reinterpret_cast<float*>(ws + pl.o_off);
     c.B = batch;
     c.Hq = num_q_heads;
     c.Hkv = num_kv_heads;
     c.n_rep = n_rep;
     c.tiles = pl.tiles;
-    c.splits = pl.splits;
-    c.parts = pl.parts;
+    c.whole = pl.whole;
+    c.shares = c.max_shares = pl.max_shares;
+    c.ranked = pl.ranked;
+    c.n_pieces = pl.n_pieces;
+    c.sms = sm_count();
     c.alt = pl.alt;
-    c.ranked = pl.n_items <= kMaxRanked && static_cast<int64_t>(pl.n_items) * pl.splits * num_kv_heads > sm_count();
     c.causal = causal;
     c.max_blocks = max_blocks;
     c.num_pages = num_pages;
