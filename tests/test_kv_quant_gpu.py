@@ -809,3 +809,25 @@ def test_a_captured_batch_is_cut_by_the_lengths_of_its_replay(cuda, n_rep, new):
         want = step()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
         _check(out, lse, q, kv, bt, lens, new, 0.1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("h_kv,n_rep,new,lens", [
+    (8, 4, [60, 45, 70], [600, 1500, 70]),  # several items a worker, its pairs of warps at different ones
+    (1, 8, [130, 131], [400, 131]),
+    (8, 1, [1] * 300, list(range(1, 301))),  # 8-row items
+    (4, 2, [90] * 60, [90] * 60),            # more items than are split: pairs run on by themselves
+])
+def test_pairs_of_warps_at_different_items(cuda, dtype, h_kv, n_rep, new, lens):
+    """head_dim 256: two warps share a head, and pairs do not wait for one another."""
+    kv = _fill(cuda, 20, h_kv, 256, seed=66)
+    bt = _shared_pages(cuda, lens, 20, seed=67)
+    g = torch.Generator(device=cuda).manual_seed(12)
+    q = torch.randn(sum(new), h_kv * n_rep, 256, generator=g, device=cuda) * torch.exp2(
+        3 * torch.randn(sum(new), h_kv * n_rep, 1, generator=g, device=cuda))
+    q = q.to(DT[dtype])
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, n_rep, 0.02)
+    for _ in range(10):
+        again = _chunk(cuda, q, kv, bt, lens, new, n_rep, 0.02)
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    _check(out, lse, q, kv, bt, lens, new, 0.02)

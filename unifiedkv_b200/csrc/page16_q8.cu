@@ -370,10 +370,11 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       if constexpr (DS == 2) {  // one exponent for the whole row
+        // in the warp's own part of the buffer, as below: only the two warps wait for each other
         uint32_t* x = reinterpret_cast<uint32_t*>(s_pair + turn * NW * NT * 32);
-        x[warp * 32 + lane] = amax;
+        x[warp * NT * 128 + lane] = amax;
         meet();
-        amax = max(amax, x[(warp ^ 1) * 32 + lane]);
+        amax = max(amax, x[(warp ^ 1) * NT * 128 + lane]);
         turn ^= 1;
       }
       // exponent that brings the largest element into [2^14, 2^15); rows of zeros, or not finite, stay as they are
