@@ -18,10 +18,10 @@ struct ChunkQ8Params {
   float* lse_out;
   float* part_o;    // [parts][total_q * Hq][D]
   float* part_lse;  // [parts][total_q * Hq]
-  // How the row tiles are cut into pieces, a CTA per piece and KV head, longest row tile first.  One request: its
-  // last `whole` row tiles whole, the others in `shares` shares of their tokens each.  A batch: planned on the
-  // device from the lengths: pieces[i] = (row tile or -1, share | shares << 16), n_shares its shares; or (pieces
-  // null) all whole, and, if `ranked`, each CTA works the order out.
+  // How the row tiles are cut into pieces, a CTA per piece and KV head, longest row tile first (in a batch if
+  // `ranked`: each CTA works the order out): `whole` row tiles whole, the others in `shares` shares of their tokens
+  // each.  Or (pieces not null) planned on the device from the lengths: pieces[i] = (row tile or -1,
+  // share | shares << 16), and n_shares of each row tile.
   int2* pieces;       // [n_pieces]
   int32_t* n_shares;  // [B * tiles]
   int whole, shares, n_pieces, ranked, max_shares, sms;

@@ -276,10 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     share = piece.y & 0xffff;
     shares = piece.y >> 16;
     if (item < 0) return;  // uniform across the CTA
-  } else if (p.B == 1) {
+  } else if (item >= p.whole) {
     const int i = item - p.whole;
-    item = p.tiles - 1 - (i < 0 ? item : p.whole + i / p.shares);
-    if (i >= 0) share = i % p.shares, shares = p.shares;
+    item = p.whole + i / p.shares, share = i % p.shares, shares = p.shares;
+  }
+  if (p.B == 1) {
+    item = p.tiles - 1 - item;
   } else if (p.ranked) {
     __shared__ int s_item;
     const int n_items = p.B * p.tiles;
@@ -840,7 +842,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_q8_merge_kernel(const 
     const int tile = r / (ALT ? kBM : 2 * kBM);
     if (tile >= p.tiles) return 0;
     const int shares = p.pieces != nullptr ? __ldcg(p.n_shares + b * p.tiles + tile)
-                       : p.B == 1 && tile < p.tiles - p.whole ? p.shares : 1;
+                       : tile < p.tiles - p.whole ? p.shares : 1;
     return ALT ? 2 * shares : shares > 1 ? shares : 0;
   };
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5); first < all_rows; first += 32 * step) {

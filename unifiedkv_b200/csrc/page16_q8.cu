@@ -762,14 +762,22 @@ constexpr int kTcRows = 32;
 // zero to two full waves of CTAs whole, the rest in s shares.  Measured (32 heads, 8 KV heads, head_dim
 // 128), 1 share / chosen: 512 new tokens of 32768 732 / 389 us, 128 new of 32768 718 / 117, 2048 new of 32768
 // (256 CTAs; 144 whole, 112 in 4 shares) 1461 / 1326.
-void choose_shares(int row_tiles, int Hkv, int64_t tokens, int most, int& whole, int& shares) {
+//
+// A batch over a wide table: chunk_q8_plan_kernel, which knows the lengths, chooses.  Over a narrow one its time
+// (about 6 us, and the CTAs left over some more) is not won back: all row tiles in s shares, 2 at least
+// if they fit one wave, since the longest request sets the time.  Measured, s shares / planned: 8 x 64 new over 2048
+// tokens each 52 / 58 us, over 3900 77 / 86, over 100-3900 76 / 54; 6 x 1-333 over 170-3000 59 / 72; 4 x 64 over
+// 200-8000 73 / 55, 16 x 16 over 2000-16000 173 / 174, 16 x 32 over 8192 each 196 / 179.
+constexpr int kPlanTokens = 4096;
+void choose_shares(int row_tiles, int Hkv, int64_t tokens, int most, bool batch, int& whole, int& shares) {
   const int sms = sm_count();
   const float tiles = static_cast<float>(tokens) / 128.f;
+  const int fewest = batch && static_cast<int64_t>(row_tiles) * Hkv <= sms ? min(2, most) : 1;
   float least = 1e30f;
-  for (int w = 0; w < 3; ++w) {
+  for (int w = 0; w < (batch ? 1 : 3); ++w) {
     const int n = static_cast<int>(min(static_cast<int64_t>(row_tiles), static_cast<int64_t>(w) * sms / Hkv));
     if (w > 0 && (n == 0 || n == row_tiles)) continue;
-    for (int s = w == 0 ? 1 : 2; s <= most; ++s) {
+    for (int s = w == 0 ? fewest : 2; s <= most; ++s) {
       const float pieces = n + static_cast<float>(s) * (row_tiles - n), waves = pieces * Hkv / sms;
       const float cut = tiles / s + (s > 1 ? 11.f : 9.f), first = n > 0 ? tiles + 9.f : cut;
       const float t = fmaxf(first, (n * (tiles + 9.f) + s * (row_tiles - n) * cut) * Hkv / sms + (ceilf(waves) - waves) * cut);
@@ -778,13 +786,8 @@ void choose_shares(int row_tiles, int Hkv, int64_t tokens, int most, int& whole,
   }
 }
 
-// A batch: chunk_q8_plan_kernel, which knows the lengths, chooses, if the table is wide enough (it costs
-// about 6 us, and the CTAs left over a little).  Measured, whole / planned: 8 x 64 new over 2048 tokens each 62 / 58
-// us, over 100-3900 103 / 54, 4 x 64 over 200-8000 190 / 55, 16 x 16 over 2000-16000 282 / 174, 16 x 32 over 8192 each
-// 178 / 179.
 // Shares that a row tile may be cut into: this bounds the CTAs and the parts' memory (8 x 256 rows per SM).  A
 // share is 512 tokens at least.
-constexpr int kPlanTokens = 2048;
 int most_shares(int64_t ctas, int64_t tokens, int most) {
   const int64_t sms = sm_count();
   const int64_t s = ctas <= sms / 2 ? 2 * sms / ctas : ctas <= 2 * sms ? max(static_cast<int64_t>(4), 4 * sms / ctas) : 1;
@@ -811,17 +814,17 @@ Plan make_plan(int B, int total_q, int Hkv, int n_rep, int D, int max_q, int max
     const int64_t tokens = static_cast<int64_t>(max_blocks) * kPage;
     pl.n_pieces = pl.n_items;
     pl.max_shares = most_shares(ctas, tokens, pl.alt ? kMaxParts / 2 : kMaxParts);
-    if (B == 1 && pl.n_items > 0) {
-      choose_shares(pl.n_items, Hkv, tokens, pl.max_shares, pl.whole, pl.max_shares);
-      pl.n_pieces = pl.whole + (pl.n_items - pl.whole) * pl.max_shares;
-    } else if (pl.n_items > 0 && pl.n_items <= kMaxRanked && pl.max_shares > 1 && tokens >= kPlanTokens) {
+    if (pl.n_items <= 0) {
+      pl.max_shares = 1;
+    } else if (B > 1 && tokens >= kPlanTokens && pl.n_items <= kMaxRanked && pl.max_shares > 1) {
       pl.planned = 1;
       pl.n_pieces = min(pl.n_items * pl.max_shares, pl.n_items + 2 * sms / Hkv);
       pl.shares_off = up256(sizeof(int2) * pl.n_pieces);
       pl.bytes = pl.lse_off = pl.shares_off + up256(sizeof(int32_t) * pl.n_items);
     } else {
-      pl.max_shares = 1;
-      pl.ranked = pl.n_items <= kMaxRanked && ctas > sms;
+      choose_shares(pl.n_items, Hkv, tokens, pl.max_shares, B > 1, pl.whole, pl.max_shares);
+      pl.n_pieces = pl.whole + (pl.n_items - pl.whole) * pl.max_shares;
+      pl.ranked = B > 1 && pl.n_items <= kMaxRanked && static_cast<int64_t>(pl.n_pieces) * Hkv > sms;
     }
     const int parts = pl.max_shares * (pl.alt ? 2 : 1);
     if (parts > 1) {
