@@ -35,13 +35,16 @@
 //    them.  With very many items (long chunks) no item is split: worker w takes items
 //    w, w + W, ... and there is no merge.
 //  * Loads: a ring of NS pages per warp filled by cp.async, no block barriers.
+//  * head_dim 256: two warps share a head, half its dimensions each, and exchange scores through shared
+//    memory: half the accumulators a warp (15 x 7-58 new over 58-174 tokens 118 us with one warp a
+//    head, 91 so; decode, latency-bound, unchanged).
 //
 // Measured (8 KV heads, head_dim 128, 32 query heads, bf16; attention / combine kernel): 32 requests
 // of 4K-32K tokens 153 / 9 us for 972 MB (6.4 TB/s, 97 % of the measured copy rate), one of 131072
-// 53 / 10 us for 271 MB; 16 requests with 16 rows each 59 / 11 us for 200 MB, where the two MMA
+// 53 / 8.5 us for 271 MB; 16 requests with 16 rows each 59 / 10.5 us for 200 MB, where the two MMA
 // columns of tiles double the arithmetic per byte and issue slots bound it.  What mattered most
 // beside the MMA layout was code size: exact power-of-two factors in place of scalbnf took 16 rows
-// from 94 to 69 us a call and head_dim 256 from 43 to 38.
+// from 94 to 69 us a call (now 67) and head_dim 256 from 43 to 38.
 #include <math.h>
 #include <string.h>
 

@@ -281,9 +281,11 @@ def paged_chunk_prefill_q8(q_chunk: torch.Tensor, kv: QuantPagedKV, block_table:
     when ``causal`` is false), the chunk's own K and V being in the cache already
     (``quantize_append``).  Chunks of one or a few tokens (drafts) and long ones both
     run here.  Lengths as lists (past_lens, chunk_lens) or device tensors (cu_seqlens_q
-    [B+1], seqlens_k [B] = past + chunk, with max_seqlen_q the longest chunk; longer
-    chunks than that are cut).  A query that sees no token gives zeros (lse -inf); rows
-    behind the last sequence are not written.  ``softmax_scale`` defaults to head_dim^-0.5.
+    [B+1], seqlens_k [B] = past + chunk, with max_seqlen_q the longest chunk; of a longer
+    chunk the rows past that may be left unwritten).  A query that sees no token gives
+    zeros (lse -inf); rows behind the last sequence are not written.  ``softmax_scale``
+    defaults to head_dim^-0.5.  A row's last bits depend on the other lengths of its
+    batch, as they decide how its tokens are shared out.
     """
     what = "prefill"
     total = int(q_chunk.shape[0])
