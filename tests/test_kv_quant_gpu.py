@@ -831,3 +831,40 @@ def test_pairs_of_warps_at_different_items(cuda, dtype, h_kv, n_rep, new, lens):
         again = _chunk(cuda, q, kv, bt, lens, new, n_rep, 0.02)
         assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
     _check(out, lse, q, kv, bt, lens, new, 0.02)
+
+
+@pytest.mark.parametrize("new,lens", [
+    ([9 + i % 4 for i in range(600)], [12 + i % 50 for i in range(600)]),        # 36 to 48 rows
+    ([30 + i % 121 for i in range(200)], [150 + i % 31 for i in range(200)]),    # one to three row tiles
+])
+def test_more_row_tiles_than_are_put_in_order(cuda, new, lens):
+    kv = _fill(cuda, 20, 1, 64, seed=68)
+    bt = _shared_pages(cuda, lens, 20, seed=69)
+    q = torch.randn(sum(new), 4, 64, device=cuda, generator=torch.Generator(device=cuda).manual_seed(13)).bfloat16()
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, 4, 0.125)
+    _check(out, lse, q, kv, bt, lens, new, 0.125)
+
+
+def test_two_batches_at_once_on_two_streams(cuda):
+    """Batches cut on the device, each with its own plan and parts, side by side."""
+    from unifiedkv_b200.kv_quant import paged_chunk_prefill_q8
+    runs = []
+    for i, lens in enumerate(([5000, 300, 4500], [100, 5100, 64])):
+        new = [40, 33, 50]
+        kv = _fill(cuda, 20, 2, 128, seed=70 + i)
+        bt, sk, cu = _shared_pages(cuda, lens, 20, seed=72), _i32(cuda, lens), _cu(cuda, new)
+        q = torch.randn(sum(new), 4, 128, device=cuda).bfloat16()
+
+        def step(q=q, kv=kv, bt=bt, sk=sk, cu=cu):
+            return paged_chunk_prefill_q8(q, kv, bt, softmax_scale=0.1, n_rep=2, cu_seqlens_q=cu, seqlens_k=sk, max_seqlen_q=50)
+        runs.append((step, step()))
+    streams = [torch.cuda.Stream(cuda) for _ in runs]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(runs[i][0]())
+    torch.cuda.synchronize()
+    for (_, want), got in zip(runs, outs):
+        assert all(torch.equal(want, g) for g in got)
