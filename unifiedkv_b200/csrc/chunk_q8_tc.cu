@@ -30,16 +30,16 @@
 //    1439 us for 2048 new of 32768 tokens against 1440 with none: the special function
 //    unit is not what bounds the kernel.)
 //  * The K/V tiles of row tiles are cut into shares where that fills the SMs better, a CTA
-//    each: by the host for one request, by chunk_q8_plan_kernel for a batch, whose lengths
-//    only the device knows.  Shares (and the two groups when alternating) leave fp32 (o, lse)
-//    parts that chunk_q8_merge_kernel joins.
+//    each: by the host for one request and for narrow tables, else by chunk_q8_plan_kernel
+//    from the batch's lengths, which only the device knows.  Shares (and the two groups when
+//    alternating) leave fp32 (o, lse) parts that chunk_q8_merge_kernel joins.
 //  * Every wait is bounded (a poll count and 2 s); one that runs out ends in NaN rows.
 //
 // Measured (32 query heads, 8 KV heads, head_dim 128, bf16): 2048 new of 32768 tokens 1.33 ms, 801
 // TFLOP/s, 50 % of the measured cuBLAS burst (the 16-bit pages' kernel: 797); 8 x 512 over 900-16000
-// tokens 0.39 ms, 695.  Before row tiles were cut (1.45 ms) converters that store nothing took 1.35, an eighth of the MMAs 1.17:
-// the softmax chain (S, maximum, weights, P.V, next S) of two groups bounds it, and the converters'
-// stores share the shared-memory port with the MMAs' operands.
+// tokens 0.39 ms, 695.  Before row tiles were cut (1.45 ms) it took 1.35 with converters that store
+// nothing and 1.17 with an eighth of the MMAs: the softmax chain (S, maximum, weights, P.V, next S) of two
+// groups bounds it, and the converters' stores share the shared-memory port with the MMAs' operands.
 #include <type_traits>
 
 #include "chunk_q8.cuh"
