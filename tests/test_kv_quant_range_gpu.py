@@ -1,0 +1,152 @@
+"""GPU tests of attention over 8-bit pages at the edges of the number range, against the 64-bit oracle.
+
+Here a row's bound is made of the tokens that the row sees and of nothing else: what a causal mask hides, or
+what a row gives no weight to, may not move it however large it is.  With weights p (largest 1), l = sum p, and
+for each token t that the row sees
+
+  * dx_t = (d + 8) 2^-24 X_t + d 2^-38 log2(e) |scale| max|q| max|k_t|, X_t = log2(e) |scale| sum |q_i k_t,i|:
+    a score summed in fp32 over d products of q (rounded to fp16 after its row was scaled to [2^14, 2^15): off by
+    2^-25 of 2^14) and exact keys;
+  * mv_t = ln2 dx_t + 2^-21 + n 2^-27: with two exponentials of 2^-22 and sums of n weights, 16 a step, in fp32
+    (a step of the tensor cores' sums may be cut off rather than rounded: 2^-23);
+  * 2^-11 of a weight for bf16 results (half a step of fp16), 2^-22 for fp16 ones (two parts);
+  * weights end at half a step of fp16's subnormals, 2^-25, in units of 2^-11 of the row's reference (chunk kernel:
+    2^-36 of the largest weight) or of 2^-12 2^(vunit - vbyte_t) of it, vunit < vbyte_t + 8 (2^-30): both of |v_t|;
+
+an element of the result is off by at most
+  sum_t (p_t (exp(mv_t) - 1 + weight) + 2^-30) |v_t| / l + |out| sum_t p_t (exp(mv_t) - 1) / l
+and its rounding to bf16 / fp16, half a step.  The log-sum-exp moves by sum_t p_t (exp(mv_t) - 1) / l and is rounded
+to fp32 a few times.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_quant as oracle
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _i32(device, x):
+    return torch.tensor(list(x), dtype=torch.int32, device=device)
+
+
+def _cache(device, k, v, seed):
+    """Requests' rows (lists of [n, h_kv, d]) in pages of no order -> cache, table."""
+    from unifiedkv_b200.kv_quant import QuantPagedKV
+    need = [-(-len(x) // 16) for x in k]
+    rng = np.random.default_rng(seed)
+    ids = rng.permutation(sum(need) + 2)
+    h_kv, d = k[0].shape[1:]
+    out, table = [], np.zeros((len(k), max(max(need), 1)), np.int32)
+    for rows in (k, v):
+        codes = np.zeros((len(ids), 16, h_kv, d), np.uint8)
+        scales = np.zeros((len(ids), h_kv, 16), np.uint8)
+        at = 0
+        for b, x in enumerate(rows):
+            c, e = oracle.quantise(x)
+            for j in range(need[b]):
+                m = min(16, len(x) - 16 * j)
+                table[b, j] = ids[at]
+                codes[ids[at], :m] = c[16 * j:16 * j + m]
+                scales[ids[at], :, :m] = e[16 * j:16 * j + m].T
+                at += 1
+        out.append((torch.from_numpy(codes).to(device).view(torch.float8_e4m3fn), torch.from_numpy(scales).to(device)))
+    return QuantPagedKV(out[0][0], out[1][0], out[0][1], out[1][1]), torch.from_numpy(table).to(device)
+
+
+def _bounds(q, k, v, there, scale, causal, weight):
+    """q [m, h_q, d], k and v [n, h_kv, d] in 64 bits -> out, lse, and how far each may be off."""
+    m, h_q, d = q.shape
+    n, h_kv = k.shape[:2]
+    rep = h_q // h_kv
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    lse, ltol = np.full((m, h_q), -np.inf), np.zeros((m, h_q))
+    for i in range(m):
+        see = there & (np.arange(n) <= (n - m + i if causal else n - 1))
+        if not see.any():
+            continue
+        for h in range(h_q):
+            kk, vv, qq = k[see, h // rep], v[see, h // rep], q[i, h]
+            s = kk @ qq * scale
+            top = s.max()
+            p = np.exp(s - top)
+            l = p.sum()
+            size = np.log2(np.e) * abs(scale) * (np.abs(kk) @ np.abs(qq))
+            most = d * np.log2(np.e) * abs(scale) * np.abs(qq).max() * np.abs(kk).max(-1)
+            mv = np.log(2) * ((d + 8) * 2.0 ** -24 * size + 2.0 ** -38 * most) + 2.0 ** -21 + n * 2.0 ** -27
+            off = np.exp(np.minimum(s - top + mv, 700)) - p
+            out[i, h] = p @ vv / l
+            tol[i, h] = (off + weight * p + 2.0 ** -30) @ np.abs(vv) / l + np.abs(out[i, h]) * off.sum() / l
+            lse[i, h] = top + np.log(l)
+            ltol[i, h] = off.sum() / l + 2.0 ** -22 * (1 + abs(lse[i, h]))
+    return out, lse, tol, ltol
+
+
+def _check(got, lse, q, kv, bt, lens, new, scale, causal=True, empty=0.0):
+    kc, vc, ks, vs = (t.view(torch.uint8).cpu().numpy() for t in kv)
+    table, qn, g = bt.cpu().numpy(), q.double().cpu().numpy(), got.double().cpu().numpy()
+    info, at = torch.finfo(got.dtype), 0
+    weight = 2.0 ** -22 if got.dtype == torch.float16 else 2.0 ** -11
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -134  # half a step of the subnormals
+    for b, (n, m) in enumerate(zip(lens, new)):
+        k, there = oracle.request_rows(kc, ks, table[b], n)
+        v, _ = oracle.request_rows(vc, vs, table[b], n)
+        ref, ref_lse, tol, ltol = _bounds(qn[at:at + m], k, v, there, scale, causal, weight)
+        o, l = g[at:at + m], lse[at:at + m].double().cpu().numpy()
+        at += m
+        tol = tol * (1 + info.eps) + info.eps / 2 * np.abs(ref) + tiny
+        none = np.isneginf(ref_lse)
+        assert np.isnan(o[none]).all() if np.isnan(empty) else (o[none] == empty).all()
+        with np.errstate(invalid="ignore"):
+            near = np.abs(o - ref) <= tol
+        # half a step or more above the type's largest number rounds to an infinity
+        near |= (np.abs(ref) + tol >= info.max * (1 + info.eps / 4)) & np.isinf(o) & (np.sign(o) == np.sign(ref))
+        bad = ~none[..., None] & ~near
+        assert not bad.any(), (b, n, m, int(bad.sum()), np.argwhere(bad)[:4], o[bad][:4], ref[bad][:4], tol[bad][:4])
+        assert np.isneginf(l[none]).all()
+        wrong = ~none & ~(np.abs(l - np.where(none, 0, ref_lse)) <= ltol)
+        assert not wrong.any(), (b, np.argwhere(wrong)[:4], l[wrong][:4], ref_lse[wrong][:4], ltol[wrong][:4])
+
+
+def _chunk(device, q, kv, bt, lens, new, scale, causal=True):
+    from unifiedkv_b200.kv_quant import paged_chunk_prefill_q8
+    lse = torch.full(q.shape[:2], 9.0, device=device)
+    out = paged_chunk_prefill_q8(q, kv, bt, softmax_scale=scale, n_rep=q.shape[1] // kv.k_codes.shape[2], causal=causal,
+                                 cu_seqlens_q=_i32(device, np.concatenate([[0], np.cumsum(new)])),
+                                 seqlens_k=_i32(device, lens), max_seqlen_q=max(new), lse_out=lse)
+    return out, lse
+
+
+def _decode(device, q, kv, bt, lens, scale):
+    from unifiedkv_b200.kv_quant import page16_decode_attention_q8
+    lse = torch.full(q.shape[:2], 9.0, device=device)
+    return page16_decode_attention_q8(q, kv, bt, _i32(device, lens), softmax_scale=scale,
+                                      n_rep=q.shape[1] // kv.k_codes.shape[2], lse_out=lse), lse
+
+
+def _q(device, total, hq, d, dtype, seed, size=1.0):
+    g = torch.Generator(device=device).manual_seed(seed)
+    return (torch.randn(total, hq, d, generator=g, device=device) * size).to(DT[dtype])
+
+
+# ---- small queries over tiles without keys, or with keys of zeros ------------------
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [40, 150])  # 80 rows (alternating groups), 300 (two row tiles)
+def test_small_queries_over_absent_tiles_and_zero_keys(cuda, d, new):
+    rng = np.random.default_rng(d + new)
+    n = 700
+    k, v = (rng.standard_normal((n, 1, d)) for _ in (0, 1))
+    k[400:] = 0  # zeros up to and under the causal border
+    kv, bt = _cache(cuda, [k], [v], 1)
+    gone = bt.clone()
+    gone[0, 8:17] = -1  # a whole 128-token tile, and a page of the next
+    for size in (1.0, 2.0 ** -8, 2.0 ** -20, 2.0 ** -40):
+        q = _q(cuda, new, 2, d, "bf16", 3, size)
+        for table in (bt, gone):
+            _check(*_chunk(cuda, q, kv, table, [n], [new], d ** -0.5), q, kv, table, [n], [new], d ** -0.5)
+    q = _q(cuda, new, 2, d, "bf16", 4)
+    for scale in (1e-20, 1e-37):
+        _check(*_chunk(cuda, q, kv, gone, [n], [new], scale), q, kv, gone, [n], [new], scale)

@@ -652,7 +652,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       tc::tc_fence_after();
       if (k == 0) qf = s_qf[(ALT ? 0 : g * kBM) + row];
       const TileInfo& info = s_info[t % kInfo];
-      const float scale = info.scale * qf;
+      // Not below the smallest normal number: a tile whose keys are all zero or absent would bring it to 0, and a
+      // masked score of -inf times 0 is NaN.  |S| <= 2^31, so what real scores gain by this is below 2^-95.
+      const float scale = fmaxf(info.scale * qf, 1.17549435e-38f);
       const int tbase = t * kBN + sc0;
       const bool crosses = tbase + kSC - 1 > lim;
       const bool special = info.special != 0;
