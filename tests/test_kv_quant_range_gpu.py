@@ -150,3 +150,58 @@ def test_small_queries_over_absent_tiles_and_zero_keys(cuda, d, new):
     q = _q(cuda, new, 2, d, "bf16", 4)
     for scale in (1e-20, 1e-37):
         _check(*_chunk(cuda, q, kv, gone, [n], [new], scale), q, kv, gone, [n], [new], scale)
+
+
+# ---- one huge row: hidden from a query, or of no weight to it ----------------------
+def _huge_rows(n, h_kv, d, where, k_log, v_log, seed):
+    """Unit rows, but for rows `where`: keys -2^k_log along the first dimension, values of 2^v_log."""
+    rng = np.random.default_rng(seed)
+    k, v = (rng.standard_normal((n, h_kv, d)) for _ in (0, 1))
+    for t in where:
+        if k_log is not None:
+            k[t] = 0
+            k[t, :, 0] = -2.0 ** k_log
+        v[t] *= 2.0 ** v_log
+    return k, v
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,d", [(2, 64), (4, 128), (2, 256)])
+@pytest.mark.parametrize("v_log", [9, 25, 45, 68, -20, -68])
+def test_few_rows_beside_a_huge_value(cuda, dtype, hq, d, v_log):
+    """Drafted tokens: the last token's value is huge (or every other one tiny), and only the last query sees it."""
+    for n, new in ((5, 2), (100, 4), (700, 3)):
+        k, v = _huge_rows(n, 1, d, [n - 1], None, v_log, seed=n)
+        kv, bt = _cache(cuda, [k], [v], 2)
+        q = _q(cuda, new, hq, d, dtype, 5)
+        _check(*_chunk(cuda, q, kv, bt, [n], [new], d ** -0.5), q, kv, bt, [n], [new], d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,d", [(2, 64), (4, 128), (2, 256)])
+@pytest.mark.parametrize("v_log", [12, 30, 60])
+def test_decode_beside_a_huge_value_of_no_weight(cuda, dtype, hq, d, v_log):
+    lens = [5, 40, 333, 6000]
+    rows = [_huge_rows(n, 1, d, {0, n // 2, n - 2}, 13, v_log, seed=n) for n in lens]
+    kv, bt = _cache(cuda, [r[0] for r in rows], [r[1] for r in rows], 3)
+    q = _q(cuda, len(lens), hq, d, dtype, 6)
+    q[:, :, 0] = 4
+    _check(*_decode(cuda, q, kv, bt, lens, d ** -0.5), q, kv, bt, lens, [1] * 4, d ** -0.5, empty=float("nan"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,d", [(2, 64), (4, 128), (2, 256)])
+@pytest.mark.parametrize("spread", [6.0, 14.0])
+def test_few_rows_over_values_of_every_size(cuda, dtype, hq, d, spread):
+    rng = np.random.default_rng(d)
+    lens = [3, 16, 200, 2500]
+    k = [rng.standard_normal((n, 1, d)) for n in lens]
+    v = [rng.standard_normal((n, 1, d)) * 2.0 ** np.clip(rng.standard_normal((n, 1, 1)) * spread, -33, 33) for n in lens]
+    for x in v:
+        x[::5] = 0
+    kv, bt = _cache(cuda, k, v, 4)
+    q = _q(cuda, len(lens), hq, d, dtype, 7)
+    _check(*_decode(cuda, q, kv, bt, lens, d ** -0.5), q, kv, bt, lens, [1] * 4, d ** -0.5, empty=float("nan"))
+    new = [2, 3, 4, 3]
+    q = _q(cuda, sum(new), hq, d, dtype, 8)
+    _check(*_chunk(cuda, q, kv, bt, lens, new, d ** -0.5), q, kv, bt, lens, new, d ** -0.5)

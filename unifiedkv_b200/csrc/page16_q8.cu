@@ -16,9 +16,12 @@
 //    the score in fp32, the value's scale multiplies the weight in fp32 before it is
 //    rounded to fp16 (off by 2^-11 of it at most, against 2^-8 for the bf16 output).
 //    fp16 outputs keep 11 bits themselves: their weights go in as a high and a low
-//    part, two MMAs.  Weights are kept in units of 2^(largest value scale seen so far
-//    - 12): they reach 2^15 at most, hold 11 bits down to 2^-29 of that and vanish at
-//    2^-40 of it.
+//    part, two MMAs.  Weights are kept in units of 2^(reference value scale - 12): they
+//    reach 2^15 at most.  The reference follows the pages' scales, and a page whose scales
+//    span 2^8 and more is walked once per span, so that a weight holds 11 bits down to
+//    2^-18 of the row's largest and vanishes at 2^-30 of it whatever else the page or the
+//    request holds: a huge value that a row does not see, or gives no weight to, takes
+//    nothing from it (up to a ratio of 2^72).
 //  * q is scaled per row by a power of two into [2^14, 2^15) and rounded to fp16:
 //    exact for fp16 and bf16 elements down to 2^-29 of the row's largest, and off by
 //    at most 2^-40 of it below that.
@@ -80,6 +83,9 @@ namespace {
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMaxLazy = 3.f;  // a row's reference may lag its maximum by this (log2): p <= 2^3
 constexpr int kWOff = 12;        // weights are held as p * 2^(byte - vref + 12) <= 2^15
+constexpr int kVSpan = 8;        // of the value scales that one reference serves: bytes in (vref - 8, vref]
+constexpr int kVDeep = 72;       // the reference stays within this of its highest: O * 2^72 does not overflow
+constexpr int kAllBytes = 255;
 
 struct Item {
   int b, q0, row0, n_rows, len, n_q;  // rows [row0, row0 + R) of n_rows; first packed token q0
@@ -410,12 +416,15 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
     }
-    int vref = 0;  // largest value-scale byte so far
+    int vref = 0, vtop = 0;  // value-scale byte whose unit the weights and O are in; the highest so far
+    int below = kAllBytes;   // less: the page is walked again, for its tokens with value-scale bytes up to this
 
-    for (; cs.page < cs.end; ++cs.page) {
-      load_one((it_stage + NS - 1) % NS);
-      cp_async_wait<NS - 1>();
-      __syncwarp();
+    while (cs.page < cs.end) {
+      if (below == kAllBytes) {
+        load_one((it_stage + NS - 1) % NS);
+        cp_async_wait<NS - 1>();
+        __syncwarp();
+      }
       const uint32_t sk = ring + (it_stage % NS) * STAGEB;
       const uint32_t sv = sk + TILEB, ss = sk + 2 * TILEB;
       int live;
@@ -475,9 +484,10 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
       // ---- scores, online softmax in log2 ----
       const float kf0 = q8::scale_of(kb0), kf1 = q8::scale_of(kb1);
       const bool edge = live < kPage || t0 + kPage - 1 > lim_min;
-      // Rare, and looked for with one vote: a row whose maximum outgrew its reference, a value scale above
-      // the reference so far, a value row that is not finite.
-      bool rare = max(vb0, vb1) > vref || vb0 == q8::kNanByte || vb1 == q8::kNanByte;
+      // Rare, and looked for with one vote: a row whose maximum outgrew its reference, a value scale above the
+      // reference (byte 255, not finite, among them) or far below it (byte 0, zeros, apart), a further walk.
+      bool rare = max(vb0, vb1) > vref || static_cast<int>(min(vb0 - 1u, vb1 - 1u) & 0x7fffffffu) < vref - kVSpan ||
+                  below < kAllBytes;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -537,11 +547,16 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
 #pragma unroll
           for (int mt = 0; mt < MT; mt += 2) load_v(mt, vr[mt / 2]);
         }
-        const int vmax = __reduce_max_sync(0xffffffffu, max(vb0, vb1));
-        if (vmax > vref) {
-          // 2^(vref - vmax); far below: nothing of the old sum is left
-          const float a = vmax - vref > 126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - (vmax - vref)) << 23);
+        // The unit follows the page's largest value scale (of the tokens not yet taken) up, or down when that is
+        // far below.  What then still lies below the span waits for another walk over the page: one unit would
+        // round those tokens' weights away, although a row may see none of the larger ones.
+        int vmax = __reduce_max_sync(0xffffffffu, max(vb0 <= below ? vb0 : 0, vb1 <= below ? vb1 : 0));
+        vmax = vmax == 0 ? vref : max(vmax, vtop - kVDeep);
+        if (vmax > vref || vmax <= vref - kVSpan) {
+          // 2^(vref - vmax), exact; far below: nothing of the old sum is left
+          const float a = vmax - vref > 126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 + vref - vmax) << 23);
           vref = vmax;
+          vtop = max(vtop, vref);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -549,6 +564,23 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[nt][mt][e] *= a;
         }
+        // (a walk's unit is at or below the last one's cut, so there are at most kVDeep / kVSpan + 1 of them)
+        const int cut = vref - kVSpan >= vtop - kVDeep ? vref - kVSpan : 0;
+        const bool later0 = vb0 > 0 && vb0 <= cut, later1 = vb1 > 0 && vb1 <= cut;
+        const bool again = __any_sync(0xffffffffu, later0 || later1);
+        if (again || below < kAllBytes) {
+          const bool out0 = later0 || vb0 > below || (vb0 == 0 && below < kAllBytes);
+          const bool out1 = later1 || vb1 > below || (vb1 == 0 && below < kAllBytes);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s[nt][e] = out0 ? -INFINITY : s[nt][e];
+              s[nt][2 + e] = out1 ? -INFINITY : s[nt][2 + e];
+            }
+          }
+        }
+        below = again ? cut : kAllBytes;
       }
       const int ve0 = vb0 - vref + kWOff + 127, ve1 = vb1 - vref + kWOff + 127;
       const float vf0 = ve0 > 0 ? __uint_as_float(static_cast<uint32_t>(ve0) << 23) : 0.f;
@@ -596,7 +628,10 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         }
       }
       __syncwarp();
-      it_stage = it_stage + 1 == NS ? 0 : it_stage + 1;
+      if (below == kAllBytes) {
+        it_stage = it_stage + 1 == NS ? 0 : it_stage + 1;
+        ++cs.page;
+      }
     }
 
     // ---- finish the item (or this worker's share of it) ----
