@@ -205,3 +205,54 @@ def test_few_rows_over_values_of_every_size(cuda, dtype, hq, d, spread):
     new = [2, 3, 4, 3]
     q = _q(cuda, sum(new), hq, d, dtype, 8)
     _check(*_chunk(cuda, q, kv, bt, lens, new, d ** -0.5), q, kv, bt, lens, new, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [40, 150])
+@pytest.mark.parametrize("k_log,v_log,at", [
+    (None, 20, -3), (None, 45, -3),  # hidden from all but the last three queries
+    (13, 18, 0), (13, 45, 0),        # seen by all, of no weight
+    (30, 0, -3), (28, 45, -60),
+    (None, -40, 3),                  # tiny beside its tile
+])
+def test_chunks_beside_a_huge_row(cuda, dtype, d, new, k_log, v_log, at):
+    n = 300
+    k, v = _huge_rows(n, 1, d, [at % n], k_log, v_log, seed=9)
+    kv, bt = _cache(cuda, [k], [v], 5)
+    q = _q(cuda, new, 2, d, dtype, 10)
+    q[:, :, 0] = 4
+    _check(*_chunk(cuda, q, kv, bt, [n], [new], d ** -0.5), q, kv, bt, [n], [new], d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunks_cut_into_shares_beside_a_huge_row(cuda, dtype, d):
+    """Some CTAs of a row tile meet the huge rows, others do not; pages that are not there, NaN rows."""
+    lens, new = [5000, 300, 4100], [40, 3, 50]
+    rows = [_huge_rows(n, 2, d, [n // 3, n - 2], 13, 40, seed=n) for n in lens]
+    kv, bt = _cache(cuda, [r[0] for r in rows], [r[1] for r in rows], 6)
+    bt[0, 100:120] = -1
+    bt[0, 104] = 1 << 20
+    q = _q(cuda, sum(new), 8, d, dtype, 11)
+    q[:, :, 0] = 4
+    out, lse = _chunk(cuda, q, kv, bt, lens, new, d ** -0.5)
+    _check(out, lse, q, kv, bt, lens, new, d ** -0.5)
+    page, slot = int(bt[2, (4100 - 20) // 16]), (4100 - 20) % 16  # a NaN value row that the last 20 queries see
+    kv.v_codes.view(torch.uint8)[page, slot] = 0x7F
+    kv.v_scales[page, :, slot] = 255
+    got, _ = _chunk(cuda, q, kv, bt, lens, new, d ** -0.5)
+    assert torch.isnan(got[-20:]).all() and torch.equal(got[:-20], out[:-20])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunks_over_scales_that_move(cuda, dtype, d):
+    """Values that grow and shrink from tile to tile by less than the span that fp16 holds exactly."""
+    rng = np.random.default_rng(d)
+    n, new = 900, 150
+    log = np.concatenate([np.full(128, x) for x in (0, 5, 9, 2, -1, 8, 9, 3)])[:n, None, None]
+    k, v = rng.standard_normal((n, 1, d)) * 2.0 ** (log / 4), rng.standard_normal((n, 1, d)) * 2.0 ** log
+    kv, bt = _cache(cuda, [k], [v], 7)
+    q = _q(cuda, new, 2, d, dtype, 12)
+    _check(*_chunk(cuda, q, kv, bt, [n], [new], 0.05), q, kv, bt, [n], [new], 0.05)

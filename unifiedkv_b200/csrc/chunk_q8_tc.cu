@@ -15,8 +15,10 @@
 //    tiles deep.  A key takes its scale relative to the tile's largest, which joins the
 //    softmax scale: one multiplier per tile.  A value takes its scale relative to a
 //    reference that follows the largest seen (64 above it stays in range; O is rescaled in
-//    the rare case that it moves).  Both are exact down to 2^-15 of the largest scale
-//    (values: 2^-21) and lose at most 2^-33 of the largest element below that.
+//    the rare case that it moves).  Both are exact down to 2^-15 of the reference.  Where a
+//    CTA meets a smaller scale (but for 0, that of rows of zeros) its rows are computed once
+//    more, from the codes, in fp32 without tensor cores: a key or value 2^15 times the others
+//    takes nothing from rows that do not see it, at some hundred times the time.
 //  * q goes to fp16 with a power of two per row that brings the row into [2^14, 2^15):
 //    exact down to 2^-29 of the row's largest element, off by 2^-40 of it below.
 //  * Groups A and B of 8 softmax warps, 128 rows each, 2 threads per row.  The MMA warp
@@ -64,6 +66,7 @@ constexpr int kMaxPages = 1024;       // block-table entries staged in shared me
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescale = 4.f, kWOff = 11.f;  // weights <= 2^4, held times 2^11
 constexpr int kVHead = 6;                      // values are held as code * 2^(byte - vref), byte <= vref + 6
+constexpr int kExact = 15;                     // codes times 2^-15 are fp16 numbers still
 
 // What a K/V tile's scales come to, worked out once by the scale warp: for the converters a factor per row
 // (fp16 bits), for the softmax warps the rest.  A ring of 4; a slot is free again once P.V of its tile is done.
@@ -139,6 +142,19 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
       "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
       "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate));
+}
+
+// What a CTA needs to look at its scales once more (look: not all lie near one another), and to start over where they
+// are too far apart for fp16 operands (wide).
+struct Keep {
+  int look, wide, vmin, vmax, item, tile0, n_tiles, share, shares;
+};
+
+// s += x, with what the additions so far rounded away in c.
+__device__ __forceinline__ void add_exactly(float& s, float& c, float x) {
+  const float y = x - c, t = s + y;
+  c = (t - s) - y;
+  s = t;
 }
 
 struct RowTile {
@@ -247,6 +263,154 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_q8_plan_kernel(const __gri
   for (int i = total + tid; i < p.n_pieces; i += kPlanThreads) p.pieces[i] = make_int2(-1, 0);
 }
 
+// Whether a tile of keys, or all the values, have scales too far apart; but for rows of zeros, NaN, and rows that are not
+// there.  16 lanes a tile: keys of its 8 pages, then values.
+template <bool ALT>
+__device__ __forceinline__ void look_at_scales(const ChunkQ8Params& p, volatile Keep* keep) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = static_cast<int>(blockIdx.x % p.Hkv);
+  const RowTile rt = row_tile<ALT>(p, keep->item);
+  const int32_t* bt_row = p.bt + static_cast<int64_t>(rt.b) * p.bt_sb;
+  const int tile0 = keep->tile0, end = tile0 + keep->n_tiles;
+  int vmax = 0, vmin = 255;
+  for (int t0 = tile0 + 2 * warp; t0 < end; t0 += 4 * kGroupWarps) {
+    const int t = t0 + lane / 16, first = t * kBN + lane % 8 * kPage, live = min(rt.kv_end, end * kBN) - first;
+    const int page = live > 0 ? q8::page_of(bt_row, first / kPage, p.max_blocks, p.num_pages) : -1;
+    int most = 0, least = 255;
+    if (page >= 0) {
+      const uint8_t* s = (lane & 8 ? p.vs : p.ks) + page * p.scale_stride + hkv * kPage;
+      for (int i = 0; i < min(live, kPage); ++i) {
+        const int b = __ldg(s + i);
+        if (b != q8::kNanByte) most = max(most, b);
+        if (b != 0) least = min(least, b);
+      }
+    }
+    if (lane & 8) {
+      vmax = max(vmax, most), vmin = min(vmin, least);
+      most = 0;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+    }
+    if (least < most - kExact) keep->wide = 1;
+  }
+  vmax = __reduce_max_sync(0xffffffffu, vmax), vmin = __reduce_min_sync(0xffffffffu, vmin);
+  if (lane == 0) {
+    atomicMax(const_cast<int*>(&keep->vmax), vmax);
+    atomicMin(const_cast<int*>(&keep->vmin), vmin);
+  }
+}
+
+// The work of a CTA that met scales too far apart: a row's tokens one after the other, in fp32 from the codes; kR rows a
+// warp, D / 32 columns a lane.  (What it needs it works out anew: the tensor-core path has no registers to keep it in.)
+template <typename T, int D, bool ALT>
+__device__ __forceinline__ void exact_rows(const ChunkQ8Params& p, const volatile Keep* keep) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile0 = keep->tile0, n_tiles = keep->n_tiles, share = keep->share, hkv = static_cast<int>(blockIdx.x % p.Hkv);
+  const bool whole = !ALT && keep->shares == 1;
+  const RowTile rt = row_tile<ALT>(p, keep->item);
+  const int len = __ldg(p.lens + rt.b);
+  const int32_t* bt_row = p.bt + static_cast<int64_t>(rt.b) * p.bt_sb;
+  const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
+  constexpr int kR = 2, C = D / 32;
+  for (int first = warp * kR; first < Layout<D, ALT>::kQTiles * kBM && rt.row0 + first < rt.n_rows; first += 2 * kGroupWarps * kR) {
+    float x[kR][C], f[kR], m[kR], sum[kR], sum_c[kR], acc[kR][C], acc_c[kR][C];
+    int last[kR], end = 0;
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const int rr = min(rt.row0 + first + i, rt.n_rows - 1);
+      const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(rt.q0 + rr / p.n_rep) * p.q_st +
+                     static_cast<int64_t>(hkv * p.n_rep + rr % p.n_rep) * p.q_sh + lane * C;
+      uint32_t amax = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        x[i][c] = Elem<T>::to_f(src[c]);
+        amax = max(amax, __float_as_uint(x[i][c]) & 0x7fffffffu);
+      }
+      amax = __reduce_max_sync(0xffffffffu, amax);
+      int qe = static_cast<int>(amax >> 23) - 127 - 14;
+      qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[i][c] *= __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
+      f[i] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
+      last[i] = min(min(p.causal ? len - rt.n_q + rr / p.n_rep : len - 1, rt.kv_end - 1), (tile0 + n_tiles) * kBN - 1);
+      end = max(end, last[i] + 1);
+      m[i] = -INFINITY;
+      sum[i] = sum_c[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[i][c] = acc_c[i][c] = 0.f;
+    }
+    for (int t = tile0 * kBN; t < end; ++t) {
+      const int page = q8::page_of(bt_row, t / kPage, p.max_blocks, p.num_pages);
+      if (page < 0) continue;
+      const int64_t at = page * p.page_stride + (static_cast<int64_t>(t % kPage) * p.Hkv + hkv) * D + lane * C;
+      const int64_t sat = page * p.scale_stride + hkv * kPage + t % kPage;
+      uint32_t kw, vw;
+      if constexpr (C == 4) {
+        kw = __ldg(reinterpret_cast<const uint32_t*>(p.kc + at));
+        vw = __ldg(reinterpret_cast<const uint32_t*>(p.vc + at));
+      } else {
+        kw = __ldg(reinterpret_cast<const uint16_t*>(p.kc + at));
+        vw = __ldg(reinterpret_cast<const uint16_t*>(p.vc + at));
+      }
+      // values times 2^-16, so that their sums stay in range
+      const float kf = q8::scale_of(__ldg(p.ks + sat)), vf = q8::scale_of(__ldg(p.vs + sat)) * 0x1p-16f;
+      float kx[4], vx[4];
+      auto floats = [](uint32_t w, float* y) {
+        uint32_t lo, hi;
+        q8::e4m3x4_to_f16x4(w, lo, hi);
+        const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+        y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
+      };
+      floats(kw, kx);
+      floats(vw, vx);
+#pragma unroll
+      for (int i = 0; i < kR; ++i) {
+        if (t > last[i]) continue;  // the same for the whole warp
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) dot += x[i][c] * kx[c];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        const float s = dot * fminf(f[i] * kf, 3.4028235e38f), mn = fmaxf(m[i], s), mu = mn == -INFINITY ? 0.f : mn;
+        const float a = fast_exp2(m[i] - mu), w = fast_exp2(s - mu);
+        m[i] = mn;
+        sum[i] *= a, sum_c[i] *= a;
+        add_exactly(sum[i], sum_c[i], w);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          acc[i][c] *= a, acc_c[i][c] *= a;
+          add_exactly(acc[i][c], acc_c[i][c], w * (vx[c] * vf));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const int rr = rt.row0 + first + i;
+      if (rr >= rt.n_rows || first + i >= Layout<D, ALT>::kQTiles * kBM) continue;
+      const bool none = sum[i] == 0.f;
+      const float inv = none ? 0.f : 1.f / sum[i], lse = none ? -INFINITY : (m[i] + log2f(sum[i])) * kLn2;
+      const int64_t o = static_cast<int64_t>(rt.q0 + rr / p.n_rep) * p.Hq + hkv * p.n_rep + rr % p.n_rep;
+      if (whole) {
+#pragma unroll
+        for (int c = 0; c < C; c += 2)
+          *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + o * D + lane * C + c) =
+              pack2<T>(none ? p.empty : acc[i][c] * inv * 65536.f, none ? p.empty : acc[i][c + 1] * inv * 65536.f);
+        if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = lse;
+      } else {  // alternating groups leave two parts: this is the first, and the second is empty
+#pragma unroll
+        for (int part = 0; part < (ALT ? 2 : 1); ++part) {
+          const int64_t po = (ALT ? 2 * share + part : share) * all_rows + o;
+#pragma unroll
+          for (int c = 0; c < C; ++c) p.part_o[po * D + lane * C + c] = part == 0 ? acc[i][c] * inv * 65536.f : 0.f;
+          if (lane == 0) p.part_lse[po] = part == 0 ? lse : -INFINITY;
+        }
+      }
+    }
+  }
+}
+
 template <typename T, int D, bool ALT>
 __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_constant__ ChunkQ8Params p) {
   using L = Layout<D, ALT>;
@@ -257,7 +421,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   constexpr int kBarCount = 4 * kRing + 7 + 2 * kInfo;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBarCount);
-  static_assert((kBarCount + 1) * 8 <= 256, "barrier area");
+  volatile Keep* keep = reinterpret_cast<Keep*>(tmem_slot + 2);
+  static_assert((kBarCount + 1) * 8 + sizeof(Keep) <= 256, "barrier area");
   TileInfo* s_info = reinterpret_cast<TileInfo*>(smem + L::kInfoOff);
   float* s_mx = reinterpret_cast<float*>(smem + L::kMx);
   float* s_l = reinterpret_cast<float*>(smem + L::kL);
@@ -329,6 +494,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       tc::mbar_init(info_full(i), 32u);
       tc::mbar_init(info_free(i), 1u);
     }
+    keep->look = keep->wide = keep->vmax = 0;
+    keep->vmin = 255;
+    keep->item = item;
+    keep->tile0 = tile0;
+    keep->n_tiles = n_tiles;
+    keep->share = share;
+    keep->shares = shares;
     tc::mbar_init(q_full, 32u * 2 * kGroupWarps);
     for (int g = 0; g < 2; ++g) {
       tc::mbar_init(s_full(g), 1u);
@@ -405,6 +577,42 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < N; ++i) fetch(h, i);
     }
+    // Are there scales below what the operands hold exactly?  Mostly all keys' bytes lie in 16 around that of a token in
+    // the middle, and all values' too: then there are none.  (Here, while the first codes are on their way, the look
+    // costs nothing that shows; 8 x 512 new tokens take 389 us, 397 to 408 with it in the softmax warps, 398 to 402 in a
+    // warp of its own that follows the tiles.)
+    {
+      const int tokens = min(rt.kv_end - tile0 * kBN, n_tiles * kBN), n_pages = (tokens + kPage - 1) / kPage;
+      const int mid = n_pages > 0 ? page_at(n_pages / 2) : -1;
+      const uint8_t *ksp = p.ks + hkv * kPage, *vsp = p.vs + hkv * kPage;
+      const int kref = mid < 0 ? 0 : __ldg(ksp + mid * p.scale_stride), vref = mid < 0 ? 0 : __ldg(vsp + mid * p.scale_stride);
+      constexpr uint32_t kAll = 0x01010101u;
+      uint32_t far = min(kref, vref) < 8 || max(kref, vref) > 246 ? ~0u : 0u;
+      auto bytes_far = [&](const uint4& x, int ref, int live) {  // a byte + 8 - ref: 0 to 15, or an upper bit is set
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        if (live < kPage) {  // rows behind the last count as the one in the middle
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int n = min(max(live - 4 * v, 0), 4);
+            const uint32_t there = n == 4 ? ~0u : (1u << (8 * n)) - 1;
+            w[v] = (w[v] & there) | (ref * kAll & ~there);
+          }
+        }
+        const uint32_t add = (8 - ref) * kAll;
+        far |= (w[0] + add) | (w[1] + add) | (w[2] + add) | (w[3] + add);
+      };
+#pragma unroll 2
+      for (int i = ct; i < n_pages; i += 32 * kConvWarps) {
+        const int page = page_at(i);
+        if (page >= 0) {
+          const uint4 kw = __ldg(reinterpret_cast<const uint4*>(ksp + page * p.scale_stride));
+          const uint4 vw = __ldg(reinterpret_cast<const uint4*>(vsp + page * p.scale_stride));
+          bytes_far(kw, kref, tokens - i * kPage);
+          bytes_far(vw, vref, tokens - i * kPage);
+        }
+      }
+      if ((far & 0xf0 * kAll) != 0) keep->look = 1;
+    }
     bool ok = true;
     for (int t = 0; ok && t < n_tiles; ++t) {
       const TileInfo& info = s_info[t % kInfo];
@@ -462,6 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(v_full(t)) : "memory");
     }
     cp_async_wait<0>();
+    asm volatile("bar.sync 10, %0;\n" ::"n"(32 * (2 * kGroupWarps + kConvWarps)) : "memory");  // with the softmax warps
   } else if (warp >= kMmaWarp) {
     // =================== MMA issue, scales (the first two warps of the group) ===================
     regs_dec<kRegsMma>();
@@ -652,9 +861,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       tc::tc_fence_after();
       if (k == 0) qf = s_qf[(ALT ? 0 : g * kBM) + row];
       const TileInfo& info = s_info[t % kInfo];
-      // Not below the smallest normal number: a tile whose keys are all zero or absent would bring it to 0, and a
-      // masked score of -inf times 0 is NaN.  |S| <= 2^31, so what real scores gain by this is below 2^-95.
-      const float scale = fmaxf(info.scale * qf, 1.17549435e-38f);
+      // Not below the smallest normal number, 2^-126: a tile whose keys are all zero or absent would bring it to 0, and
+      // a masked score of -inf times 0 is NaN.  |S| <= 2^31, so what real scores gain by this is below 2^-95.
+      const float scale = fmaf(info.scale, qf, 0x1p-126f);
       const int tbase = t * kBN + sc0;
       const bool crosses = tbase + kSC - 1 > lim;
       const bool special = info.special != 0;
@@ -814,6 +1023,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
     if (valid && half == 0) {
       if (!whole) p.part_lse[part * all_rows + o] = lse;
       else if (p.lse_out != nullptr) p.lse_out[o] = lse;
+    }
+    asm volatile("bar.sync 10, %0;\n" ::"n"(32 * (2 * kGroupWarps + kConvWarps)) : "memory");  // with the converters: keep->look is final
+    if (keep->look != 0) {
+      look_at_scales<ALT>(p, keep);
+      asm volatile("bar.sync 11, %0;\n" ::"n"(32 * 2 * kGroupWarps) : "memory");
+      if (keep->wide != 0 || keep->vmin < keep->vmax - kExact) exact_rows<T, D, ALT>(p, keep);  // over what was stored above
     }
   }
   // the merge may be scheduled from here on; it waits for this grid itself
