@@ -256,3 +256,21 @@ def test_chunks_over_scales_that_move(cuda, dtype, d):
     kv, bt = _cache(cuda, [k], [v], 7)
     q = _q(cuda, new, 2, d, dtype, 12)
     _check(*_chunk(cuda, q, kv, bt, [n], [new], 0.05), q, kv, bt, [n], [new], 0.05)
+
+
+# ---- queries that are not finite ----------------------------------------------------
+@pytest.mark.parametrize("d,new", [(64, 3), (128, 3), (256, 3), (64, 60), (128, 60), (128, 200)])
+def test_infinite_queries_give_nan(cuda, d, new):
+    """A score of inf or -inf in every token is no softmax: NaN, also where all of them are -inf."""
+    rng = np.random.default_rng(d)
+    n = new + 30
+    k, v = np.abs(rng.standard_normal((n, 1, d))) + 0.5, rng.standard_normal((n, 1, d))
+    kv, bt = _cache(cuda, [k], [v], 8)
+    q = _q(cuda, new, 2, d, "bf16", 13)
+    clean, clean_lse = _chunk(cuda, q, kv, bt, [n], [new], 0.1)
+    q[0, 0, 3], q[1, 1, 5], q[2, 0, 7] = -float("inf"), float("inf"), float("nan")
+    out, lse = _chunk(cuda, q, kv, bt, [n], [new], 0.1)
+    for i, h in ((0, 0), (1, 1), (2, 0)):
+        assert torch.isnan(out[i, h]).all(), (i, h)
+        out[i, h], lse[i, h] = clean[i, h], clean_lse[i, h]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)

@@ -332,7 +332,7 @@ __device__ __forceinline__ void exact_rows(const ChunkQ8Params& p, const volatil
       int qe = static_cast<int>(amax >> 23) - 127 - 14;
       qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[i][c] *= __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
+      for (int c = 0; c < C; ++c) x[i][c] *= q8::q_factor(amax, qe);
       f[i] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
       last[i] = min(min(p.causal ? len - rt.n_q + rr / p.n_rep : len - 1, rt.kv_end - 1), (tile0 + n_tiles) * kBN - 1);
       end = max(end, last[i] + 1);
@@ -832,10 +832,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
         for (int u = 0; u < 8; ++u) amax = max(amax, __float_as_uint(Elem<T>::to_f(x[u])) & 0x7fffffffu);
 #pragma unroll
         for (int o = 1; o < CPR; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        // rows of zeros, or not finite, stay as they are
+        // rows of zeros stay as they are, rows that are not finite become NaN
         int qe = static_cast<int>(amax >> 23) - 127 - 14;
         qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
-        const float inv = __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
+        const float inv = q8::q_factor(amax, qe);
         uint32_t y[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) y[u] = pack2<__half>(Elem<T>::to_f(x[2 * u]) * inv, Elem<T>::to_f(x[2 * u + 1]) * inv);

@@ -386,10 +386,11 @@ __global__ void __launch_bounds__(NW * 32, 1) q8_attend_kernel(Q8Params p) {
         amax = max(amax, x[(warp ^ 1) * NT * 128 + lane]);
         turn ^= 1;
       }
-      // exponent that brings the largest element into [2^14, 2^15); rows of zeros, or not finite, stay as they are
+      // exponent that brings the largest element into [2^14, 2^15); rows of zeros stay as they are, rows that are not
+      // finite become NaN
       int qe = static_cast<int>(amax >> 23) - 127 - 14;
       qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - qe) << 23);
+      const float inv = q8::q_factor(amax, qe);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const T* x = e + 4 * s;

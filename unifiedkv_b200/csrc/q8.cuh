@@ -35,6 +35,12 @@ __device__ __forceinline__ int scale_byte(uint32_t amax) {
   return min(max(e, -127), 119) + 127;
 }
 
+// 2^-qe, what a query row whose largest magnitude has the bits `amax` is multiplied by.  A row with an infinity or a NaN
+// becomes NaN: whatever its scores are (with one infinite element all of them can be -inf), they have no softmax.
+__device__ __forceinline__ float q_factor(uint32_t amax, int qe) {
+  return __uint_as_float(amax >= 0x7f800000u ? 0x7fc00000u : static_cast<uint32_t>(127 - qe) << 23);
+}
+
 // Two floats -> two e4m3 codes (a in the low byte), round to nearest even.
 __device__ __forceinline__ uint32_t to_e4m3x2(float a, float b) {
   uint16_t r;
