@@ -274,3 +274,17 @@ def test_infinite_queries_give_nan(cuda, d, new):
         assert torch.isnan(out[i, h]).all(), (i, h)
         out[i, h], lse[i, h] = clean[i, h], clean_lse[i, h]
     assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+# ---- values at the top of the range --------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_the_largest_values_do_not_overflow(cuda, d):
+    """Every value the largest that the format holds: so is the mean, however many parts it is joined from."""
+    n, top = 3000, 448 * 2.0 ** 119
+    rng = np.random.default_rng(d)
+    kv, bt = _cache(cuda, [rng.standard_normal((n, 2, d))], [np.full((n, 2, d), top)], 9)
+    q = _q(cuda, 1, 4, d, "bf16", 14)
+    _check(*_decode(cuda, q, kv, bt, [n], 0.1), q, kv, bt, [n], [1], 0.1)
+    for new in (3, 60, 200):
+        q = _q(cuda, new, 4, d, "bf16", 15)
+        _check(*_chunk(cuda, q, kv, bt, [n], [new], 0.1), q, kv, bt, [n], [new], 0.1)

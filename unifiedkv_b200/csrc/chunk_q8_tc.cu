@@ -1086,8 +1086,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_q8_merge_kernel(const 
         W += w[u];
       }
       for (int s = 16; s > 0; s >>= 1) W += __shfl_xor_sync(0xffffffffu, W, s);
+      const bool blank = M == -INFINITY && !nan;
+      const float inv = nan ? __int_as_float(0x7fc00000) : blank ? 0.f : 1.f / W;
 #pragma unroll
       for (int u = 0; u < kMaxParts / 32; ++u) {
+        w[u] *= inv;  // before the sums: those of the largest values stay in range
         const int n = min(32, parts - u * 32);
 #pragma unroll 4
         for (int i = 0; i < n; ++i) {
@@ -1097,11 +1100,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_q8_merge_kernel(const 
           for (int k = 0; k < C; ++k) a[k] += wi * src[k];
         }
       }
-      const bool blank = M == -INFINITY && !nan;
-      const float inv = nan ? __int_as_float(0x7fc00000) : blank ? 0.f : 1.f / W;
       T* dst = static_cast<T*>(p.out) + o * D + lane * C;
 #pragma unroll
-      for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(blank ? p.empty : a[k] * inv, blank ? p.empty : a[k + 1] * inv);
+      for (int k = 0; k < C; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack2<T>(blank ? p.empty : a[k], blank ? p.empty : a[k + 1]);
       if (lane == 0 && p.lse_out != nullptr) p.lse_out[o] = nan ? inv : M == -INFINITY ? -INFINITY : M + logf(W);
     }
   }

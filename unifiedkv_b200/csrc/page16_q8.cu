@@ -755,10 +755,11 @@ __global__ void __launch_bounds__(kCombMaxWarps * 32) q8_combine_kernel(Q8Params
   __syncthreads();
   L = lane < nw ? s_red[1][lane] : 0.f;
   for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  const float inv = M == -INFINITY ? 0.f : 1.f / L;  // into the weights: sums of the largest values stay in range
   float a[C] = {};
 #pragma unroll 8
   for (int i = warp; i < n; i += nw) {
-    const float w = s_w[i];
+    const float w = s_w[i] * inv;
     const float* src = p.part_o + part(i) * D + lane * C;
     float x[C];
     if constexpr (C == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(kCombMaxWarps * 32) q8_combine_kernel(Q8Params
     float y = 0.f;
 #pragma unroll 8
     for (int w = 0; w < nw; ++w) y += s_acc[w][d];
-    static_cast<T*>(p.out)[o * D + d] = Elem<T>::from_f(M == -INFINITY ? p.empty : y / L);
+    static_cast<T*>(p.out)[o * D + d] = Elem<T>::from_f(M == -INFINITY ? p.empty : y);
   }
   if (tid == 0 && p.lse_out != nullptr) p.lse_out[o] = M == -INFINITY ? -INFINITY : M + logf(L);
 }
