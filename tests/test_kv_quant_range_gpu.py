@@ -288,3 +288,38 @@ def test_the_largest_values_do_not_overflow(cuda, d):
     for new in (3, 60, 200):
         q = _q(cuda, new, 4, d, "bf16", 15)
         _check(*_chunk(cuda, q, kv, bt, [n], [new], 0.1), q, kv, bt, [n], [new], 0.1)
+
+
+# ---- the second part of fp16 weights -------------------------------------------------
+def _cancelling(n, h_kv, d, seed):
+    """Values in pairs of opposite sign, keys small: the result is small beside the values, and a weight that was
+    rounded to 11 bits shows."""
+    rng = np.random.default_rng(seed)
+    k, v = rng.standard_normal((n, h_kv, d)) * 0.25, rng.standard_normal((n, h_kv, d))
+    v[1::2] = -v[:n // 2 * 2:2]
+    return k, v
+
+
+@pytest.mark.parametrize("d,new,n", [(64, 1, 16), (128, 1, 32), (256, 1, 16), (64, 3, 40), (64, 40, 60), (128, 40, 64),
+                                     (128, 150, 160)])
+def test_weights_of_fp16_results_keep_both_parts(cuda, d, new, n):
+    k, v = _cancelling(n, 1, d, seed=d)
+    kv, bt = _cache(cuda, [k], [v], 10)
+    q = _q(cuda, new, 2, d, "fp16", 16, 0.25)
+    _check(*_chunk(cuda, q, kv, bt, [n], [new], d ** -0.5), q, kv, bt, [n], [new], d ** -0.5)
+
+
+# ---- softmax scales of zero and below -------------------------------------------------
+@pytest.mark.parametrize("hq,h_kv,d,new,lens", [(4, 2, 128, [60, 9], [160, 30]), (4, 2, 64, [3, 1], [20, 500]),
+                                                (4, 1, 256, [20, 5], [90, 5]), (1, 1, 64, [1] * 4200, [3] * 4200)])
+def test_log_sums_of_scales_of_zero_and_below(cuda, hq, h_kv, d, new, lens):
+    rng = np.random.default_rng(d)
+    if len(lens) > 100:  # more requests than are split between workers, over two pages
+        kv, bt = _cache(cuda, [rng.standard_normal((32, h_kv, d))], [rng.standard_normal((32, h_kv, d))], 11)
+        bt = bt[0][torch.arange(len(lens), device=cuda) % 2][:, None].contiguous()
+    else:
+        kv, bt = _cache(cuda, *([rng.standard_normal((n, h_kv, d)) for n in lens] for _ in (0, 1)), 11)
+        bt[0, 1] = -1  # a page that is not there
+    q = _q(cuda, sum(new), hq, d, "bf16", 17)
+    for scale in (-0.1, 0.0):
+        _check(*_chunk(cuda, q, kv, bt, lens, new, scale), q, kv, bt, lens, new, scale)
