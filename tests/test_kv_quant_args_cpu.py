@@ -1,0 +1,17 @@
+"""CPU tests of how the 8-bit cache's Python side takes its arguments."""
+import pytest
+import torch
+
+from unifiedkv_b200 import kv_quant
+
+
+def test_64_bit_numbers_do_not_wrap():
+    ids = torch.tensor([[0, 2 ** 32 + 1, -2 ** 32, 2 ** 31, -1]])
+    got = kv_quant._table(ids, "x")
+    assert got.dtype == torch.int32 and got[0, 0] == 0 and got[0, 1] == 2 ** 31 - 1 == got[0, 3]
+    assert got[0, 2] < 0 and got[0, 4] == -1
+    got = kv_quant._int32(torch.tensor([2 ** 32 + 1, 5]), "x", "seqlens", 2)
+    assert got.tolist() == [2 ** 31 - 1, 5]
+    same = torch.tensor([1, 2], dtype=torch.int32)
+    assert kv_quant._int32(same, "x", "seqlens", 2) is same
+    assert kv_quant._int32(torch.tensor([1, 2], dtype=torch.int16), "x", "seqlens", 2).tolist() == [1, 2]

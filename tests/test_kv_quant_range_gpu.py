@@ -323,3 +323,22 @@ def test_log_sums_of_scales_of_zero_and_below(cuda, hq, h_kv, d, new, lens):
     q = _q(cuda, sum(new), hq, d, "bf16", 17)
     for scale in (-0.1, 0.0):
         _check(*_chunk(cuda, q, kv, bt, lens, new, scale), q, kv, bt, lens, new, scale)
+
+
+# ---- 64-bit page ids and lengths -------------------------------------------------------
+def test_ids_and_lengths_past_32_bits(cuda):
+    """Page ids of a 64-bit table that lie outside the pool stay outside it when they are narrowed."""
+    from unifiedkv_b200.kv_quant import dequantize_pages, quantize_append
+    rng = np.random.default_rng(0)
+    kv, bt = _cache(cuda, [rng.standard_normal((48, 2, 64))], [rng.standard_normal((48, 2, 64))], 12)
+    before = [t.view(torch.uint8).clone() for t in kv]
+    x = torch.ones(2, 2, 64, device=cuda, dtype=torch.bfloat16)
+    far = torch.tensor([[2 ** 32 + 1], [-2 ** 32]], device=cuda)
+    quantize_append(kv, x, x, far, _i32(cuda, [1, 1]))
+    quantize_append(kv, x, x, torch.zeros(2, 1, dtype=torch.int64, device=cuda),
+                    torch.tensor([2 ** 32 + 1, 2 - 2 ** 32], device=cuda))
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, kv))
+    k, v = dequantize_pages(kv, far, _i32(cuda, [0, 4, 8]), 8)
+    assert (k == 0).all() and (v == 0).all()
+    out, lse = _decode(cuda, x, kv, far, [4, 4], 0.1)
+    assert torch.isnan(out).all() and torch.isneginf(lse).all()

@@ -88,11 +88,19 @@ def _check_device(what: str, dev: torch.device, *tensors: Optional[torch.Tensor]
             raise RuntimeError(f"{what}_shape_unsupported:device_{t.device}")
 
 
+def _narrow(t: torch.Tensor) -> torch.Tensor:
+    """int32; 64-bit numbers past its range stay far out (a page id out of the pool stays out of it)."""
+    if t.dtype is torch.int32:
+        return t
+    if t.dtype is torch.int64:
+        t = t.clamp(-2 ** 30, 2 ** 31 - 1)
+    return t.to(torch.int32)
+
+
 def _int32(t: torch.Tensor, what: str, name: str, numel: int) -> torch.Tensor:
     if t.numel() != numel:
         raise RuntimeError(f"{what}_shape_unsupported:{name}")
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+    t = _narrow(t)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -101,8 +109,7 @@ def _table(t: torch.Tensor, what: str, batch: Optional[int] = None) -> torch.Ten
         raise RuntimeError(f"{what}_shape_unsupported:block_table_rank")
     if batch is not None and t.shape[0] != batch:
         raise RuntimeError(f"{what}_shape_unsupported:block_table_batch")
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+    t = _narrow(t)
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
