@@ -15,3 +15,14 @@ def test_64_bit_numbers_do_not_wrap():
     same = torch.tensor([1, 2], dtype=torch.int32)
     assert kv_quant._int32(same, "x", "seqlens", 2) is same
     assert kv_quant._int32(torch.tensor([1, 2], dtype=torch.int16), "x", "seqlens", 2).tolist() == [1, 2]
+
+
+def test_numbers_of_the_host_are_refused_in_a_capture(monkeypatch):
+    import contextlib
+    kv_quant._refuse_capture("x", torch.device("cpu"))
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    kv_quant._refuse_capture("x", torch.device("cuda:0"))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="^x_unavailable:host_numbers_in_capture$"):
+        kv_quant._refuse_capture("x", torch.device("cuda:0"))

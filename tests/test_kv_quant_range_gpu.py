@@ -342,3 +342,30 @@ def test_ids_and_lengths_past_32_bits(cuda):
     assert (k == 0).all() and (v == 0).all()
     out, lse = _decode(cuda, x, kv, far, [4, 4], 0.1)
     assert torch.isnan(out).all() and torch.isneginf(lse).all()
+
+
+# ---- lengths that the host holds --------------------------------------------------------
+def test_calls_with_numbers_of_the_host_refuse_a_capture(cuda):
+    """Their copies to the device could not be replayed; the capture around them goes on."""
+    from unifiedkv_b200.kv_quant import QuantPagedKVPool, paged_chunk_prefill_q8
+    pool = QuantPagedKVPool(16, 1, 2, 64, device=cuda, n_total=4)
+    kv = pool.layer(0)
+    bt = torch.arange(4, dtype=torch.int32, device=cuda)[None]
+    q = _q(cuda, 5, 4, 64, "bf16", 18)
+    x = torch.ones(2, 20, 64, device=cuda, dtype=torch.bfloat16)
+    calls = [lambda: paged_chunk_prefill_q8(q, kv, bt, [9], [5], n_rep=2), lambda: pool.write_kv_to_blocks(0, [0, 1], x, x),
+             lambda: pool.write_one_token(0, 1, 4, x[:, :1], x[:, :1]), lambda: pool.read_kv_from_blocks(0, [0, 1], 20)]
+    for call in calls[1:] + calls[:1]:
+        call()
+    want = calls[0]()
+    torch.cuda.synchronize()
+    cu, lens = _i32(cuda, [0, 5]), _i32(cuda, [14])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in calls:
+            with pytest.raises(RuntimeError, match="_unavailable:host_numbers_in_capture$"):
+                call()
+        out = paged_chunk_prefill_q8(q, kv, bt, n_rep=2, cu_seqlens_q=cu, seqlens_k=lens, max_seqlen_q=5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)

@@ -29,8 +29,11 @@ more times larger than its neighbours can be lost where the row hardly looks at 
 A page id outside the pool (-1 as of an offloaded page, or past its end) is never
 touched: tokens on such a page are not written, read back as zeros, and are left out of
 attention.  Every call runs on the current stream of its tensors' device without
-synchronising with the host, and takes its scratch from torch's allocator, so that it
-can be captured in a CUDA graph and two graphs never share scratch.
+synchronising with the host, and takes its scratch from torch's allocator.  Calls whose
+lengths and tables are device tensors can be captured in a CUDA graph, and two graphs
+never share scratch.  Those that take them as Python numbers (``past_lens`` and
+``chunk_lens``, the pool's page I/O) copy them to the device when they are called, which
+no graph can replay: they refuse to be captured.
 """
 from __future__ import annotations
 
@@ -86,6 +89,14 @@ def _check_device(what: str, dev: torch.device, *tensors: Optional[torch.Tensor]
     for t in tensors:
         if t is not None and t.device != dev:
             raise RuntimeError(f"{what}_shape_unsupported:device_{t.device}")
+
+
+def _refuse_capture(what: str, dev: torch.device) -> None:
+    """For calls that copy the host's numbers: a graph would copy again from memory that is gone."""
+    if dev.type == "cuda":
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what}_unavailable:host_numbers_in_capture")
 
 
 def _narrow(t: torch.Tensor) -> torch.Tensor:
@@ -287,7 +298,7 @@ def paged_chunk_prefill_q8(q_chunk: torch.Tensor, kv: QuantPagedKV, block_table:
     Query i of a chunk of n sees the tokens t <= len - n + i of its request (every token
     when ``causal`` is false), the chunk's own K and V being in the cache already
     (``quantize_append``).  Chunks of one or a few tokens (drafts) and long ones both
-    run here.  Lengths as lists (past_lens, chunk_lens) or device tensors (cu_seqlens_q
+    run here.  Lengths as lists (past_lens, chunk_lens; not in a graph capture) or device tensors (cu_seqlens_q
     [B+1], seqlens_k [B] = past + chunk, with max_seqlen_q the longest chunk; of a longer
     chunk the rows past that may be left unwritten).  A query that sees no token gives
     zeros (lse -inf); rows behind the last sequence are not written.  ``softmax_scale``
@@ -307,6 +318,7 @@ def paged_chunk_prefill_q8(q_chunk: torch.Tensor, kv: QuantPagedKV, block_table:
         for x in chunk_lens:
             cu.append(cu[-1] + x)
         dev = q_chunk.device
+        _refuse_capture(what, dev)
         cu_seqlens_q = torch.tensor(cu, dtype=torch.int32).to(dev, non_blocking=True)
         seqlens_k = torch.tensor([p + c for p, c in zip(past_lens, chunk_lens)], dtype=torch.int32).to(dev, non_blocking=True)
         max_q = max(chunk_lens, default=0)
@@ -376,6 +388,7 @@ class QuantPagedKVPool(PagedKVPool):
 
     def write_kv_to_blocks(self, layer_id: int, block_ids: List[int], K: torch.Tensor, V: torch.Tensor):
         """K, V [h_kv, seq, d] -> pages ``block_ids`` in order, quantised."""
+        _refuse_capture("q8_pool", self.device)
         n = min(int(K.shape[1]), len(block_ids) * self.B)
         if n == 0:
             return
@@ -385,12 +398,14 @@ class QuantPagedKVPool(PagedKVPool):
 
     def write_one_token(self, layer_id: int, block_id: int, pos_in_block: int, k_tok: torch.Tensor,
                         v_tok: torch.Tensor):
+        _refuse_capture("q8_pool", self.device)
         quantize_append(self.layer(layer_id), k_tok.to(self.device).transpose(0, 1),
                         v_tok.to(self.device).transpose(0, 1), self._row(int(block_id))[None],
                         self._row(int(pos_in_block) + 1))
 
     def read_kv_from_blocks(self, layer_id: int, block_ids: List[int], seq_len: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """Pages -> K, V [h_kv, seq_len, d] of ``out_dtype``."""
+        _refuse_capture("q8_pool", self.device)
         n = max(0, min(int(seq_len), len(block_ids) * self.B))
         K = torch.empty(self.num_kv_heads, n, self.head_dim, dtype=self.out_dtype, device=self.device)
         V = torch.empty_like(K)
