@@ -26,3 +26,25 @@ def test_numbers_of_the_host_are_refused_in_a_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="^x_unavailable:host_numbers_in_capture$"):
         kv_quant._refuse_capture("x", torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("failing", [1, 2, 3, 4])
+def test_pool_allocates_again_after_running_out_of_memory(monkeypatch, failing):
+    """Whichever of the four tensors did not fit, the next access allocates the pool anew."""
+    pool = kv_quant.QuantPagedKVPool(16, 2, 2, 64, device="cpu", n_total=3)
+    made = [0]
+
+    def once(fn):
+        def make(*args, **kw):
+            made[0] += 1
+            if made[0] == failing:
+                raise torch.OutOfMemoryError("no room")
+            return fn(*args, **kw)
+        return make
+    monkeypatch.setattr(torch, "zeros", once(torch.zeros))
+    monkeypatch.setattr(torch, "zeros_like", once(torch.zeros_like))
+    with pytest.raises(torch.OutOfMemoryError):
+        pool.layer(0)
+    assert not pool.is_allocated
+    kv = pool.layer(1)
+    assert [tuple(x.shape) for x in kv] == [(3, 16, 2, 64)] * 2 + [(3, 2, 16)] * 2

@@ -356,10 +356,11 @@ class QuantPagedKVPool(PagedKVPool):
     def ensure_allocated(self) -> None:
         if self.is_allocated:
             return
-        super().ensure_allocated()
         shape = (self.num_layers, self.N_total, self.num_kv_heads, self.B)
-        self._k_scales = torch.zeros(shape, dtype=torch.uint8, device=self.device)
-        self._v_scales = torch.zeros_like(self._k_scales)
+        k_scales = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+        v_scales = torch.zeros_like(k_scales)
+        super().ensure_allocated()  # last: with its codes the pool counts as allocated
+        self._k_scales, self._v_scales = k_scales, v_scales
 
     def release_if_empty(self) -> bool:
         if not super().release_if_empty():
