@@ -185,7 +185,7 @@ def dequantize_pages(kv: QuantPagedKV, block_table: torch.Tensor, cu_seqlens: to
     to the host.  The values are exact in fp32 and bf16; fp16 rounds values below its
     normal range and overflows above 65504.  Tokens without a page read as zeros.
     ``out``: a pair of equally strided tensors to fill (unit stride of head_dim, other
-    strides multiples of 16 bytes); rows behind the last sequence keep what they held.
+    strides multiples of 16 bytes; no two elements in one place); rows behind the last sequence keep what they held.
     """
     what = "q8_dequantize"
     lib = _lib.lib()  # raises page16_native_unavailable when the library is missing
@@ -211,6 +211,8 @@ def dequantize_pages(kv: QuantPagedKV, block_table: torch.Tensor, cu_seqlens: to
         s = k.stride()
         if s[2] != 1 or s[0] % per or s[1] % per or v.stride() != s or k.data_ptr() % 16 or v.data_ptr() % 16:
             raise RuntimeError(f"{what}_shape_unsupported:out_layout")
+        if (s[0] == 0 and total > 1) or (s[1] == 0 and h_kv > 1) or (total > 0 and k.data_ptr() == v.data_ptr()):
+            raise RuntimeError(f"{what}_shape_unsupported:out_overlap")
     _check_device(what, dev, *kv, bt, cu, st, k, v)
     if dev.index != _device():  # the library launches on the current device
         with torch.cuda.device(dev):
