@@ -62,3 +62,14 @@ def test_readback_refuses_outputs_that_overlap():
     both = torch.zeros(4, 2, 2, 64)  # K and V side by side are two places
     with pytest.raises(RuntimeError, match="tensors_not_on_cuda"):
         kv_quant.dequantize_pages(kv, bt, cu, 4, out=(both[:, 0], both[:, 1]))
+
+
+def test_a_token_outside_its_page_is_refused():
+    """It would be skipped in silence: the 16-bit pool raises, too."""
+    pool = kv_quant.QuantPagedKVPool(16, 1, 2, 64, device="cpu", n_total=3)
+    x = torch.zeros(2, 1, 64)
+    for block, pos in ((0, 16), (0, -1), (3, 0), (-1, 0)):
+        with pytest.raises(RuntimeError, match=f"^q8_pool_shape_unsupported:slot_{block}_{pos}$"):
+            pool.write_one_token(0, block, pos, x, x)
+    with pytest.raises(RuntimeError, match="tensors_not_on_cuda"):
+        pool.write_one_token(0, 2, 15, x, x)

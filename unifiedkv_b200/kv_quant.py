@@ -402,6 +402,8 @@ class QuantPagedKVPool(PagedKVPool):
     def write_one_token(self, layer_id: int, block_id: int, pos_in_block: int, k_tok: torch.Tensor,
                         v_tok: torch.Tensor):
         _refuse_capture("q8_pool", self.device)
+        if not (0 <= int(block_id) < self.N_total and 0 <= int(pos_in_block) < self.B):
+            raise RuntimeError(f"q8_pool_shape_unsupported:slot_{block_id}_{pos_in_block}")
         quantize_append(self.layer(layer_id), k_tok.to(self.device).transpose(0, 1),
                         v_tok.to(self.device).transpose(0, 1), self._row(int(block_id))[None],
                         self._row(int(pos_in_block) + 1))
