@@ -54,9 +54,8 @@ def test_readback_refuses_outputs_that_overlap():
     codes, scales = torch.zeros(3, 16, 2, 64, dtype=torch.float8_e4m3fn), torch.zeros(3, 2, 16, dtype=torch.uint8)
     kv = kv_quant.QuantPagedKV(codes, codes.clone(), scales, scales.clone())
     bt, cu = torch.zeros(1, 3, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32)
-    x = torch.zeros(4, 2, 64)
-    for out in ((x, x), (x[:1].expand(4, 2, 64), x[:1].clone().expand(4, 2, 64)),
-                (x[:, :1].expand(4, 2, 64), x[:, :1].clone().expand(4, 2, 64))):
+    x, y = torch.zeros(4, 2, 64), torch.zeros(4, 2, 64)
+    for out in ((x, x), (x[:1].expand(4, 2, 64), y[:1].expand(4, 2, 64)), (x[:, :1].expand(4, 2, 64), y[:, :1].expand(4, 2, 64))):
         with pytest.raises(RuntimeError, match="^q8_dequantize_shape_unsupported:out_overlap$"):
             kv_quant.dequantize_pages(kv, bt, cu, 4, out=out)
     both = torch.zeros(4, 2, 2, 64)  # K and V side by side are two places
