@@ -147,7 +147,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
 // What a CTA needs to look at its scales once more (look: not all lie near one another), and to start over where they
 // are too far apart for fp16 operands (wide).
 struct Keep {
-  int look, wide, vmin, vmax, item, tile0, n_tiles, share, shares;
+  int look, stuck, wide, vmin, vmax, item, tile0, n_tiles, share, shares;
 };
 
 // s += x, with what the additions so far rounded away in c.
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
   constexpr int kBarCount = 4 * kRing + 7 + 2 * kInfo;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBarCount);
   volatile Keep* keep = reinterpret_cast<Keep*>(tmem_slot + 2);
-  static_assert((kBarCount + 1) * 8 + sizeof(Keep) <= 256, "barrier area");
+  static_assert((kBarCount + 1) * 8 + sizeof(Keep) <= 248, "barrier area");
   TileInfo* s_info = reinterpret_cast<TileInfo*>(smem + L::kInfoOff);
   float* s_mx = reinterpret_cast<float*>(smem + L::kMx);
   float* s_l = reinterpret_cast<float*>(smem + L::kL);
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       tc::mbar_init(info_full(i), 32u);
       tc::mbar_init(info_free(i), 1u);
     }
-    keep->look = keep->wide = keep->vmax = 0;
+    keep->look = keep->stuck = keep->wide = keep->vmax = 0;
     keep->vmin = 255;
     keep->item = item;
     keep->tile0 = tile0;
@@ -792,6 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
         }
       }
     }
+    if (warp == kMmaWarp && !ok) keep->stuck = 1;
   } else {
     // =================== softmax ===================
     regs_inc<kRegsSoftmax>();
@@ -1030,6 +1031,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_q8_kernel(const __grid_cons
       asm volatile("bar.sync 11, %0;\n" ::"n"(32 * 2 * kGroupWarps) : "memory");
       if (keep->wide != 0 || keep->vmin < keep->vmax - kExact) exact_rows<T, D, ALT>(p, keep);  // over what was stored above
     }
+  }
+  if (warp == kMmaWarp && keep->stuck != 0) {  // a wait ran out: the MMAs under way end before their TMEM is given back
+    const uint32_t drained = smem_u32(smem + L::kBars + 248);
+    if (lane == 0) {
+      tc::mbar_init(drained, 1u);
+      tc::fence_mbar_init();
+      tc::mma_commit(drained);
+    }
+    __syncwarp();
+    tc::mbar_wait(drained, 0);
   }
   // the merge may be scheduled from here on; it waits for this grid itself
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
