@@ -18,7 +18,8 @@
 //    the rare case that it moves).  Both are exact down to 2^-15 of the reference.  Where a
 //    CTA meets a smaller scale (but for 0, that of rows of zeros) its rows are computed once
 //    more, from the codes, in fp32 without tensor cores: a key or value 2^15 times the others
-//    takes nothing from rows that do not see it, at some hundred times the time.
+//    takes nothing from rows that do not see it, but time (2048 new of 32768 tokens 98 ms with
+//    one such value per head, 1.35 ms without).
 //  * q goes to fp16 with a power of two per row that brings the row into [2^14, 2^15):
 //    exact down to 2^-29 of the row's largest element, off by 2^-40 of it below.
 //  * Groups A and B of 8 softmax warps, 128 rows each, 2 threads per row.  The MMA warp
@@ -302,23 +303,33 @@ __device__ __forceinline__ void look_at_scales(const ChunkQ8Params& p, volatile 
   }
 }
 
-// The work of a CTA that met scales too far apart: a row's tokens one after the other, in fp32 from the codes; kR rows a
-// warp, D / 32 columns a lane.  (What it needs it works out anew: the tensor-core path has no registers to keep it in.)
+// The work of a CTA that met scales too far apart: two rows a warp, page by page, in fp32 from the codes.  For the dot
+// products and the values a lane has D / 32 columns; the 2 x 16 sums of a page are exchanged so that lane 16 i + j has row
+// i's of token j.  (What it needs it works out anew: the tensor-core path has no registers to keep it in.)
 template <typename T, int D, bool ALT>
 __device__ __forceinline__ void exact_rows(const ChunkQ8Params& p, const volatile Keep* keep) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int C = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = lane / 16;
   const int tile0 = keep->tile0, n_tiles = keep->n_tiles, share = keep->share, hkv = static_cast<int>(blockIdx.x % p.Hkv);
   const bool whole = !ALT && keep->shares == 1;
   const RowTile rt = row_tile<ALT>(p, keep->item);
   const int len = __ldg(p.lens + rt.b);
   const int32_t* bt_row = p.bt + static_cast<int64_t>(rt.b) * p.bt_sb;
   const int64_t all_rows = static_cast<int64_t>(p.total_q) * p.Hq;
-  constexpr int kR = 2, C = D / 32;
-  for (int first = warp * kR; first < Layout<D, ALT>::kQTiles * kBM && rt.row0 + first < rt.n_rows; first += 2 * kGroupWarps * kR) {
-    float x[kR][C], f[kR], m[kR], sum[kR], sum_c[kR], acc[kR][C], acc_c[kR][C];
-    int last[kR], end = 0;
+  auto codes = [](const uint8_t* src, float* y) {  // C of them
+    uint32_t w;
+    if constexpr (C == 4) w = __ldg(reinterpret_cast<const uint32_t*>(src));
+    else w = __ldg(reinterpret_cast<const uint16_t*>(src));
+    uint32_t lo, hi;
+    q8::e4m3x4_to_f16x4(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
+  };
+  for (int first = 2 * warp; first < Layout<D, ALT>::kQTiles * kBM && rt.row0 + first < rt.n_rows; first += 4 * kGroupWarps) {
+    float x[2][C], acc[2][C], acc_c[2][C], f = 0.f;
+    int last[2];
 #pragma unroll
-    for (int i = 0; i < kR; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const int rr = min(rt.row0 + first + i, rt.n_rows - 1);
       const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(rt.q0 + rr / p.n_rep) * p.q_st +
                      static_cast<int64_t>(hkv * p.n_rep + rr % p.n_rep) * p.q_sh + lane * C;
@@ -327,70 +338,82 @@ __device__ __forceinline__ void exact_rows(const ChunkQ8Params& p, const volatil
       for (int c = 0; c < C; ++c) {
         x[i][c] = Elem<T>::to_f(src[c]);
         amax = max(amax, __float_as_uint(x[i][c]) & 0x7fffffffu);
+        acc[i][c] = acc_c[i][c] = 0.f;
       }
       amax = __reduce_max_sync(0xffffffffu, amax);
       int qe = static_cast<int>(amax >> 23) - 127 - 14;
       qe = (amax == 0 || amax >= 0x7f800000u) ? 0 : max(qe, -100);
 #pragma unroll
       for (int c = 0; c < C; ++c) x[i][c] *= q8::q_factor(amax, qe);
-      f[i] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
+      if (mine == i) f = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + qe) << 23);
       last[i] = min(min(p.causal ? len - rt.n_q + rr / p.n_rep : len - 1, rt.kv_end - 1), (tile0 + n_tiles) * kBN - 1);
-      end = max(end, last[i] + 1);
-      m[i] = -INFINITY;
-      sum[i] = sum_c[i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < C; ++c) acc[i][c] = acc_c[i][c] = 0.f;
     }
-    for (int t = tile0 * kBN; t < end; ++t) {
-      const int page = q8::page_of(bt_row, t / kPage, p.max_blocks, p.num_pages);
+    float m = -INFINITY, sum = 0.f, sum_c = 0.f;  // of row `mine`; the sum over this lane's tokens
+    for (int t0 = tile0 * kBN; t0 <= max(last[0], last[1]); t0 += kPage) {
+      const int page = q8::page_of(bt_row, t0 / kPage, p.max_blocks, p.num_pages);
       if (page < 0) continue;
-      const int64_t at = page * p.page_stride + (static_cast<int64_t>(t % kPage) * p.Hkv + hkv) * D + lane * C;
-      const int64_t sat = page * p.scale_stride + hkv * kPage + t % kPage;
-      uint32_t kw, vw;
-      if constexpr (C == 4) {
-        kw = __ldg(reinterpret_cast<const uint32_t*>(p.kc + at));
-        vw = __ldg(reinterpret_cast<const uint32_t*>(p.vc + at));
-      } else {
-        kw = __ldg(reinterpret_cast<const uint16_t*>(p.kc + at));
-        vw = __ldg(reinterpret_cast<const uint16_t*>(p.vc + at));
+      const int64_t at = page * p.page_stride + static_cast<int64_t>(hkv) * D + lane * C, step = static_cast<int64_t>(p.Hkv) * D;
+      const int64_t sat = page * p.scale_stride + hkv * kPage + lane % 16;
+      float s[32];
+#pragma unroll
+      for (int j = 0; j < kPage; ++j) {
+        float kx[4];
+        codes(p.kc + at + j * step, kx);
+        s[j] = s[16 + j] = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[j] += x[0][c] * kx[c], s[16 + j] += x[1][c] * kx[c];
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+        for (int j = 0; j < o; ++j) {
+          const float give = lane & o ? s[j] : s[j + o], stay = lane & o ? s[j + o] : s[j];
+          s[j] = stay + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      }
+      const bool seen = t0 + lane % 16 <= (mine ? last[1] : last[0]);
+      const float score = seen ? s[0] * fminf(f * q8::scale_of(__ldg(p.ks + sat)), 3.4028235e38f) : -INFINITY;
+      float mn = score;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mn = fmaxf(m, mn);
+      const float mu = mn == -INFINITY ? 0.f : mn, a = fast_exp2(m - mu), w = fast_exp2(score - mu);
+      m = mn;
+      sum *= a, sum_c *= a;
+      add_exactly(sum, sum_c, w);
       // values times 2^-16, so that their sums stay in range
-      const float kf = q8::scale_of(__ldg(p.ks + sat)), vf = q8::scale_of(__ldg(p.vs + sat)) * 0x1p-16f;
-      float kx[4], vx[4];
-      auto floats = [](uint32_t w, float* y) {
-        uint32_t lo, hi;
-        q8::e4m3x4_to_f16x4(w, lo, hi);
-        const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-        y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y;
-      };
-      floats(kw, kx);
-      floats(vw, vx);
+      const float wv = w * (q8::scale_of(__ldg(p.vs + sat)) * 0x1p-16f);
+      float part[2][C] = {};
 #pragma unroll
-      for (int i = 0; i < kR; ++i) {
-        if (t > last[i]) continue;  // the same for the whole warp
-        float dot = 0.f;
+      for (int j = 0; j < kPage; ++j) {
+        float vx[4];
+        codes(p.vc + at + j * step, vx);
 #pragma unroll
-        for (int c = 0; c < C; ++c) dot += x[i][c] * kx[c];
+        for (int i = 0; i < 2; ++i) {
+          const float wi = __shfl_sync(0xffffffffu, wv, 16 * i + j);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        const float s = dot * fminf(f[i] * kf, 3.4028235e38f), mn = fmaxf(m[i], s), mu = mn == -INFINITY ? 0.f : mn;
-        const float a = fast_exp2(m[i] - mu), w = fast_exp2(s - mu);
-        m[i] = mn;
-        sum[i] *= a, sum_c[i] *= a;
-        add_exactly(sum[i], sum_c[i], w);
+          for (int c = 0; c < C; ++c) part[i][c] += t0 + j <= last[i] ? wi * vx[c] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float ai = __shfl_sync(0xffffffffu, a, 16 * i);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          acc[i][c] *= a, acc_c[i][c] *= a;
-          add_exactly(acc[i][c], acc_c[i][c], w * (vx[c] * vf));
+          acc[i][c] *= ai, acc_c[i][c] *= ai;
+          add_exactly(acc[i][c], acc_c[i][c], part[i][c]);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < kR; ++i) {
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float l = __shfl_sync(0xffffffffu, sum, 16 * i), top = __shfl_sync(0xffffffffu, m, 16 * i);
       const int rr = rt.row0 + first + i;
-      if (rr >= rt.n_rows || first + i >= Layout<D, ALT>::kQTiles * kBM) continue;
-      const bool none = sum[i] == 0.f;
-      const float inv = none ? 0.f : 1.f / sum[i], lse = none ? -INFINITY : (m[i] + log2f(sum[i])) * kLn2;
+      if (rr >= rt.n_rows) continue;
+      const bool none = l == 0.f;
+      const float inv = none ? 0.f : 1.f / l, lse = none ? -INFINITY : (top + log2f(l)) * kLn2;
       const int64_t o = static_cast<int64_t>(rt.q0 + rr / p.n_rep) * p.Hq + hkv * p.n_rep + rr % p.n_rep;
       if (whole) {
 #pragma unroll
