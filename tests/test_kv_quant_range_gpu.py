@@ -369,3 +369,31 @@ def test_calls_with_numbers_of_the_host_refuse_a_capture(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# ---- the exact path of the chunk kernel in other calls ------------------------------------
+@pytest.mark.parametrize("d,new", [(64, 40), (128, 40), (128, 150)])
+def test_huge_rows_without_a_causal_mask_and_in_a_replayed_graph(cuda, d, new):
+    """Every query sees every token; the huge rows come and go between replays, as do the lengths."""
+    from unifiedkv_b200.kv_quant import paged_chunk_prefill_q8
+    lens, start = [300, new + 5], [300, 260]
+    rows = [_huge_rows(n, 1, d, [n // 2], 13, 40, seed=n) for n in start]
+    kv, bt = _cache(cuda, [r[0] for r in rows], [r[1] for r in rows], 13)
+    calm, _ = _cache(cuda, *([np.random.default_rng(i).standard_normal((n, 1, d)) for n in start] for i in (0, 1)), 13)
+    q = _q(cuda, 2 * new, 2, d, "bf16", 19)
+    q[:, :, 0] = 4
+    for b in (kv, calm):
+        _check(*_chunk(cuda, q, b, bt, lens, [new, new], 0.1, causal=False), q, b, bt, lens, [new, new], 0.1, causal=False)
+    live = type(kv)(*(t.clone() for t in kv))
+    sk, cu, lse = _i32(cuda, start), _i32(cuda, [0, new, 2 * new]), torch.zeros(2 * new, 2, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_chunk_prefill_q8(q, live, bt, softmax_scale=0.1, n_rep=2, cu_seqlens_q=cu, seqlens_k=sk,
+                                     max_seqlen_q=new, lse_out=lse)
+    for source, n in ((kv, start), (calm, lens), (kv, lens), (calm, start)):
+        for a, b in zip(live, source):
+            a.copy_(b)
+        sk.copy_(_i32(cuda, n))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, lse, q, live, bt, n, [new, new], 0.1)
