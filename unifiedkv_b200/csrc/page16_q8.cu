@@ -42,12 +42,13 @@
 //    memory: half the accumulators a warp (15 x 7-58 new over 58-174 tokens 118 us with one warp a
 //    head, 91 so; decode, latency-bound, unchanged).
 //
-// Measured (8 KV heads, head_dim 128, 32 query heads, bf16; attention / combine kernel): 32 requests
-// of 4K-32K tokens 153 / 9 us for 972 MB (6.4 TB/s, 97 % of the measured copy rate), one of 131072
-// 53 / 8.5 us for 271 MB; 16 requests with 16 rows each 59 / 10.5 us for 200 MB, where the two MMA
-// columns of tiles double the arithmetic per byte and issue slots bound it.  What mattered most
-// beside the MMA layout was code size: exact power-of-two factors in place of scalbnf took 16 rows
-// from 94 to 69 us a call (now 67) and head_dim 256 from 43 to 38.
+// Measured (8 KV heads, head_dim 128, 32 query heads, bf16; attention / combine kernel, each launch by
+// itself with a cold cache): 32 requests of 4K-32K tokens 165 / 9 us for 972 MB (5.9 TB/s, 90 % of the
+// measured copy rate; the call 176 us), one of 131072 52 / 11 for 271 MB (61); 16 requests with 16 rows
+// each 67 / 13 for 200 MB (68): two MMA columns of tiles double the arithmetic per byte and leave
+// 8 warps an SM, whose dependent chains bound it (issue slots 44 % active).  What mattered most beside
+// the MMA layout was code size: exact power-of-two factors in place of scalbnf took 16 rows from 94 to
+// 69 us a call and head_dim 256 from 43 to 38.  Following the value scales costs 32 requests 3 us of 173.
 #include <math.h>
 #include <string.h>
 
@@ -798,16 +799,19 @@ constexpr int kTcRows = 32;
 // tokens: a CTA costs its tiles and about nine more (start, first tile, last output), and two more where it leaves
 // a part to be joined.
 //
-// One request: the row tiles are about as long as the table is wide, so the host chooses.  Candidates are
+// One request: the host chooses, as if it were as long as the table is wide (over a table much wider than the request
+// its shares are short).  Candidates are
 // zero to two full waves of CTAs whole, the rest in s shares.  Measured (32 heads, 8 KV heads, head_dim
 // 128), 1 share / chosen: 512 new tokens of 32768 732 / 389 us, 128 new of 32768 718 / 117, 2048 new of 32768
 // (256 CTAs; 144 whole, 112 in 4 shares) 1461 / 1326.
 //
-// A batch over a wide table: chunk_q8_plan_kernel, which knows the lengths, chooses.  Over a narrow one its time
-// (about 6 us, and the CTAs left over some more) is not won back: all row tiles in s shares, 2 at least
-// if they fit one wave, since the longest request sets the time.  Measured, s shares / planned: 8 x 64 new over 2048
-// tokens each 52 / 58 us, over 3900 77 / 86, over 100-3900 76 / 54; 6 x 1-333 over 170-3000 59 / 72; 4 x 64 over
-// 200-8000 73 / 55, 16 x 16 over 2000-16000 173 / 174, 16 x 32 over 8192 each 196 / 179.
+// A batch over a wide table: chunk_q8_plan_kernel, which knows the lengths, chooses.  Over a narrow one all row tiles
+// are cut into s shares, 2 at least if they fit one wave, since the longest request sets the time.  What decides is how
+// unequal the lengths are, which the host does not know: it goes by the table's width, below which the plan's time
+// (about 6 us, and the CTAs left over some more) is won back by very unequal lengths only.  Measured, s shares /
+// planned: 8 x 64 new over 2048 tokens each 52 / 58 us, over 3900 77 / 86, 6 x 1-333 over 170-3000 59 / 72 (but over
+// 100-3900 76 / 54); above it 4 x 64 over 200-8000 73 / 55, 16 x 16 over 2000-16000 173 / 174, 16 x 32 over 8192 each
+// 196 / 179.
 constexpr int kPlanTokens = 4096;
 void choose_shares(int row_tiles, int Hkv, int64_t tokens, int most, bool batch, int& whole, int& shares) {
   const int sms = sm_count();

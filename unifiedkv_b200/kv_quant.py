@@ -22,9 +22,14 @@ where it lies below 2^-6 * 2^e.  A row with an infinity or a NaN is stored as Na
 A token costs 2 * kv_heads * (head_dim + 1) bytes.  head_dim is 64, 128 or 256.
 
 Attention computes on the stored values: scores, softmax and sums in fp32, the products on
-fp16 operands that hold the codes exactly.  A weight is rounded to 11 bits (22 for fp16
-results) and counts as zero below 2^-36 of the largest of its row, so a value 2^25 and
-more times larger than its neighbours can be lost where the row hardly looks at it.
+fp16 operands that hold the codes exactly.  An element of q is off by at most 2^-40 of the
+largest of its row, a weight is rounded to 11 bits (22 for fp16 results) and counts as zero
+below 2^-30 of the largest of its row.  What a row does not see, or gives no weight to, takes
+nothing from it however large it is: up to a ratio of 2^72 between the values of a request
+(but rows of K or V with a largest magnitude below 2^-118 count as zeros beside larger ones).
+Scales that far apart cost time: chunks of many rows, where keys of 128 tokens or values of a
+request differ by 2^15 and more in scale, take up to a hundred times as long.  A query row
+with an infinity or a NaN gives NaN wherever it sees a token.
 
 A page id outside the pool (-1 as of an offloaded page, or past its end) is never
 touched: tokens on such a page are not written, read back as zeros, and are left out of
