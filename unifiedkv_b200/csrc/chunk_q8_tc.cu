@@ -39,7 +39,7 @@
 //  * Every wait is bounded (a poll count and 2 s); one that runs out ends in NaN rows.
 //
 // Measured (32 query heads, 8 KV heads, head_dim 128, bf16): 2048 new of 32768 tokens 1.35 to 1.37 ms
-// from box to box, 780 TFLOP/s, 48 % of the measured cuBLAS burst; 8 x 512 over 900-16000 tokens
+// from machine to machine, 780 TFLOP/s, 48 % of the measured cuBLAS burst; 8 x 512 over 900-16000 tokens
 // 0.395 ms, 690.  Before row tiles were cut (1.45 ms) it took 1.35 with converters that store
 // nothing and 1.17 with an eighth of the MMAs: the softmax chain (S, maximum, weights, P.V, next S) of two
 // groups bounds it, and the converters' stores share the shared-memory port with the MMAs' operands.

@@ -49,7 +49,7 @@
 // 8 warps an SM, whose dependent chains bound it (issue slots 44 % active).  What mattered most beside
 // the MMA layout was code size: exact power-of-two factors in place of scalbnf took 16 rows from 94 to
 // 69 us a call and head_dim 256 from 43 to 38.  Following the value scales costs 32 requests 0 to
-// 3 us of 173, from box to box.
+// 3 us of 173, from machine to machine.
 #include <math.h>
 #include <string.h>
 
